@@ -22,7 +22,7 @@ F32, F16, BF16 = 0, 1, 2
 OUTGOING, INCOMING = 0, 1
 
 # every symbol the header declares, with (restype, argtypes)
-_vp, _i32, _sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_size_t
+_vp, _i32, _i64, _sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t
 
 
 class Problem(ctypes.Structure):
@@ -120,6 +120,11 @@ SIGNATURES = {
     "ftm_bwd_ln_in_bwd": (ctypes.c_int, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp,
                                          _i32, _vp, _i32, _vp, ctypes.c_int64, _vp]),
     "ftm_static_scratch_error_word": (_vp, []),
+    "ftm_layer_norm_fwd": (ctypes.c_int, [_vp, _i32, _i64, _vp, _i32, _vp, _i32, ctypes.c_float, _vp,
+                                          _vp, _i64, _i32, _vp]),
+    "ftm_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i32]),
+    "ftm_layer_norm_bwd": (ctypes.c_int, [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp,
+                                          _i32, _vp, _sz, _i64, _i32, _vp]),
 }
 
 

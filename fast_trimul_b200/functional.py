@@ -10,9 +10,15 @@ before the input LayerNorm, and the result is multiplied by the mask again.
 On a CUDA tensor this is one C-ABI call (three sm_100a kernels) with the mask
 product, the dtype casts and the residual done inside the kernels; elsewhere it
 runs the torch formula with the reference's casts.
+
+Beside it, the other operators of a pair / single representation trunk:
+
+    layer_norm(x, weight, bias, eps)        (ops/norm.py)
 """
 
 import torch
+
+from .ops.norm import layer_norm  # noqa: F401
 
 
 def triangle_multiplication(z: torch.Tensor, params, mask: torch.Tensor = None) -> torch.Tensor:

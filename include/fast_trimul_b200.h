@@ -330,6 +330,26 @@ int ftm_trimul_fwd_static_scratch(const ftm_problem* p, const void* z, const flo
  * counterpart in the reference. */
 int* ftm_static_scratch_error_word(void);
 
+/* ---- layer norm of any width ------------------------------------------------
+ * No counterpart in the reference (its layer norms are torch's). Rows of `width`
+ * elements `x_row_stride` elements apart (the elements of a row are contiguous; a stride
+ * of 0 repeats one row); x and y have `dtype`, weight and bias (each may be NULL: 1 and
+ * 0) types of their own. y is written contiguously. stats (NULL if no backward follows):
+ * 2 * rows floats, (mean, 1 / sqrt(variance + eps)) of each row. Sums are fp32. */
+int ftm_layer_norm_fwd(const void* x, int32_t dtype, int64_t x_row_stride, const void* weight,
+                       int32_t weight_dtype, const void* bias, int32_t bias_dtype, float eps, void* y,
+                       float* stats, int64_t rows, int32_t width, ftm_stream_t stream);
+/* dx (dtype, contiguous), dweight (weight_dtype) and dbias (dbias_dtype); each may be NULL
+ * when it is not wanted, but not all three. The workspace holds per-block partial sums of
+ * dweight / dbias (not needed when both are NULL); they are added in a fixed order, so a
+ * call gives the same bits every time. */
+size_t ftm_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t width);
+int ftm_layer_norm_bwd(const void* x, int32_t dtype, int64_t x_row_stride, const void* grad,
+                       int64_t grad_row_stride, const void* weight, int32_t weight_dtype,
+                       const float* stats, void* dx, void* dweight, void* dbias, int32_t dbias_dtype,
+                       void* workspace, size_t workspace_bytes, int64_t rows, int32_t width,
+                       ftm_stream_t stream);
+
 /* ---- status -------------------------------------------------------------- */
 /* Synchronise `stream`, read the device error word of a workspace (or any err_word
  * passed to a stage) and clear it: FTM_OK, or FTM_TIMEOUT when a bounded device wait
