@@ -77,7 +77,23 @@ class ContractionLayout(ctypes.Structure):
                 ("a_mn_major", _i32), ("b_mn_major", _i32)]
 
 
+class Attention(ctypes.Structure):
+    """Mirror of ftm_attention."""
+    _fields_ = [("dtype", _i32), ("heads", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+                ("causal", _i32), ("scale", ctypes.c_float),
+                ("sequences", _i32), ("q_len", _i32), ("kv_len", _i32),
+                ("q_rows", _i64), ("kv_rows", _i64),
+                ("cu_q", _vp), ("cu_k", _vp), ("kv_lengths", _vp),
+                ("q", _vp), ("q_row_stride", _i64), ("q_head_stride", _i64),
+                ("k", _vp), ("k_row_stride", _i64), ("k_head_stride", _i64), ("k_batch_stride", _i64),
+                ("v", _vp), ("v_row_stride", _i64), ("v_head_stride", _i64), ("v_batch_stride", _i64),
+                ("key_mask", _vp), ("bias", _vp), ("bias_seqs", _i32),
+                ("bias_row_stride", _i64), ("bias_head_stride", _i64), ("bias_batch_stride", _i64),
+                ("out", _vp), ("stats", _vp)]
+
+
 _PP = ctypes.POINTER(Problem)
+_PA = ctypes.POINTER(Attention)
 _IP = ctypes.POINTER(ctypes.c_int)
 _PPL = ctypes.POINTER(PeerPlanes)
 
@@ -125,6 +141,10 @@ SIGNATURES = {
     "ftm_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i32]),
     "ftm_layer_norm_bwd": (ctypes.c_int, [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp,
                                           _i32, _vp, _sz, _i64, _i32, _vp]),
+    "ftm_attention_workspace_bytes": (_sz, [_PA, _i32]),
+    "ftm_attention_fwd": (ctypes.c_int, [_PA, _i32, _vp, _sz, _vp, _vp]),
+    "ftm_attention_bwd_workspace_bytes": (_sz, [_PA, _i32]),
+    "ftm_attention_bwd": (ctypes.c_int, [_PA, _vp, _i64, _i64, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
 

@@ -119,6 +119,9 @@ bool make_map(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base
     e[i] = 1;
   }
   for (int i = 0; i < rank - 1; ++i) s[i] = strides[i];
+  // the driver call needs a current context, which a thread that has made no runtime call yet
+  // (torch's autograd thread, when its backward begins here) does not have
+  if (cudaSetDevice(key.dev) != cudaSuccess) return false;
   const CUresult r =
       fn(m, dt, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, s, b, e,
          CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
@@ -508,6 +511,14 @@ int check_forward_args(const ftm_problem* p, const void* z, const float* mask, c
 }
 
 void set_last_launch_count(int n) { g_last_launches = n; }
+
+bool make_tensor_map(CUtensorMap* m, bool bf16, int rank, const void* base, const uint64_t* dims,
+                     const uint64_t* strides, const uint32_t* box) {
+  return make_map(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, base,
+                  dims, strides, box);
+}
+
+int device_sms(int dev) { return sm_count(dev); }
 
 }  // namespace ftm
 

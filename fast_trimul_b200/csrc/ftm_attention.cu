@@ -1,0 +1,634 @@
+// Attention forward (sm_100a): o = softmax(scale q k^T + bias) v over the keys each query
+// may see, with grouped heads, packed sequences, a key mask, an additive bias shared by a
+// run of sequences, or a cache whose lengths live on the device.
+//
+// One pass over the keys with the running maximum m and sum l of each row (fp32): a tile
+// of scores S = Q K^T (tcgen05, 128 x 128, fp32 in TMEM) is read by one thread per row,
+// turned into p = 2^(c (s - m)), written back to TMEM as a 16-bit operand over S, and
+// O += P V accumulates in TMEM. The rounding of p to the inputs' type is the only one
+// before the output's. O is rescaled only when a row's maximum grew by more than 2^8
+// (p <= 256 then, harmless in fp32 sums and 16-bit p alike), so almost never.
+//
+// Roles of a block: warps 0-3 softmax and epilogue, warp 4 TMA, warp 5 MMA. Two blocks
+// per SM (256 TMEM columns each: S / P 128, O up to 128), so one block's MMAs run under the
+// other's exponentials. A 128 x 128 tile costs 8 dim clocks of MMA and 1024 clocks of the
+// special function unit, so dim 128 is balanced between the two and smaller heads are
+// bound by the exponentials.
+//
+// Persistent grid. Packed sequences: a one-block kernel lists (sequence, tile) by
+// descending number of key tiles, so the long ones start first. Cache: the key tiles of
+// all sequences and heads are cut into equal runs, one per block; a sequence that spans
+// blocks leaves partial (O, m, l) results that a second kernel joins in a fixed order.
+#include "ftm_attention.cuh"
+
+namespace ftm {
+namespace {
+
+enum : int { KERNEL_ATTN = 4 };
+constexpr int kFwdThreads = 192;
+
+template <int DP, bool BIAS>
+struct FwdCfg {
+  static constexpr int kTile = DP / 64 * kBlk;
+  static constexpr int kStages = (DP == 64 && !BIAS) ? 2 : 1;   // K and V each
+  static constexpr int kOffK = kTile;
+  static constexpr int kOffV = kOffK + kStages * kTile;
+  static constexpr int kOffB = kOffV + kStages * kTile;
+  static constexpr int kOffBar = kOffB + (BIAS ? 2 * kBlk : 0);
+  static constexpr int kSmem = kOffBar + 256 + 1024;
+};
+
+// Cache walk: block c of n takes key tiles [c per, (c + 1) per) of the concatenation over
+// (sequence, head); `t` runs over it. Sequences are found from the lengths on the device.
+struct CacheWalk {
+  int t, end;         // this block's tiles
+  int first;          // the first tile of the block's run (partials are told apart by it)
+  int seq, head, base, tiles;   // current sequence: its first tile overall, tiles per head
+};
+
+__device__ __forceinline__ int cache_total(const AttnArgs& a, int lane) {
+  int s = 0;
+  for (int i = lane; i < a.seqs; i += 32) s += (cache_len(a, i) + kTileRows - 1) / kTileRows;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s * a.kv_heads;
+}
+__device__ __forceinline__ int cache_per_block(int total, int blocks) { return (total + blocks - 1) / blocks; }
+
+__device__ __forceinline__ void cache_start(const AttnArgs& a, int lane, CacheWalk& w) {
+  const int total = cache_total(a, lane);
+  const int per = cache_per_block(total, gridDim.x);
+  w.t = w.first = min(total, static_cast<int>(blockIdx.x) * per);
+  w.end = min(total, w.t + per);
+  // the sequence that holds tile w.t: a warp-wide scan over the lengths
+  w.seq = 0;
+  w.base = 0;
+  for (int i0 = 0; i0 < a.seqs && w.t < w.end; i0 += 32) {
+    const int i = i0 + lane;
+    const int n = i < a.seqs ? (cache_len(a, i) + kTileRows - 1) / kTileRows * a.kv_heads : 0;
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const int all = __shfl_sync(0xffffffffu, inc, 31);
+    if (w.base + all > w.t) {
+      const uint32_t hit = __ballot_sync(0xffffffffu, w.base + inc > w.t);
+      const int l = __ffs(hit) - 1;
+      w.seq = i0 + l;
+      w.base += __shfl_sync(0xffffffffu, inc - n, l);
+      break;
+    }
+    w.base += all;
+  }
+}
+
+// next run of tiles of one (sequence, head); false when the block is done
+__device__ __forceinline__ bool cache_next(const AttnArgs& a, CacheWalk& w, Item& it) {
+  if (w.t >= w.end) return false;
+  int tiles = (cache_len(a, w.seq) + kTileRows - 1) / kTileRows;
+  while (w.t >= w.base + tiles * a.kv_heads) {     // w.t < total: a later sequence holds it
+    w.base += tiles * a.kv_heads;
+    ++w.seq;
+    tiles = (cache_len(a, w.seq) + kTileRows - 1) / kTileRows;
+  }
+  const int head = (w.t - w.base) / tiles;
+  const int t0 = w.base + head * tiles;            // first tile of this (sequence, head)
+  q_item(a, w.seq, 0, head, it);
+  it.kt0 = w.t - t0;
+  const int stop = min(w.end, t0 + tiles);
+  it.kt1 = stop - t0;
+  if (it.kt0 > 0 || it.kt1 < tiles) it.slot = 2 * blockIdx.x + (w.t == w.first ? 0 : 1);
+  w.t = stop;
+  return true;
+}
+
+// the items of this block, in order; every role of the block walks the same ones
+struct FwdWalk {
+  int n;
+  CacheWalk c;
+  __device__ __forceinline__ void start(const AttnArgs& a, int lane) {
+    n = blockIdx.x;
+    if (a.walk == WALK_CACHE) cache_start(a, lane, c);
+  }
+  __device__ __forceinline__ bool next(const AttnArgs& a, Item& it) {
+    if (a.walk == WALK_CACHE) return cache_next(a, c, it);
+    if (!walk_item<false>(a, n, it)) return false;
+    n += gridDim.x;
+    return true;
+  }
+};
+
+template <int DP, bool BIAS, typename T>
+__global__ void __launch_bounds__(kFwdThreads, 2)
+attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnArgs a) {
+  using C = FwdCfg<DP, BIAS>;
+  constexpr int NS = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = smem + C::kOffK;
+  uint8_t* sV = smem + C::kOffV;
+  uint8_t* sB = smem + C::kOffB;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* k_full = q_full + 2;
+  uint64_t* k_empty = k_full + NS;
+  uint64_t* v_full = k_empty + NS;
+  uint64_t* v_empty = v_full + NS;
+  uint64_t* b_full = v_empty + NS;
+  uint64_t* b_empty = b_full + 1;
+  uint64_t* s_full = b_empty + 1;
+  uint64_t* p_ready = s_full + 1;
+  uint64_t* o_full = p_ready + 1;
+  uint64_t* drain = o_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    mbar_init(b_full, 1);
+    mbar_init(b_empty, 4);
+    mbar_init(s_full, 1);
+    mbar_init(p_ready, 4);
+    mbar_init(o_full, 1);
+    mbar_init(drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == 5) tmem_alloc(tmem_slot, 256);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dep_wait();
+  grid_dep_release();
+
+  FwdWalk walk;
+  walk.start(a, lane);
+  Item it;
+
+  if (warp == 4) {
+    // ------------------------------------------------------------------------ TMA
+    const uint32_t q_bytes = DP / 64 * 128u * (a.group * a.tq);
+    int qn = 0, kn = 0, bn = 0;
+    bool ok = true;
+    while (ok && walk.next(a, it)) {
+      if (it.kt1 <= it.kt0) continue;
+      if (lane == 0) {
+        ok = mbar_wait(q_empty, (qn & 1) ^ 1, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 1));
+        if (ok) {
+          mbar_arrive_expect_tx(q_full, q_bytes);
+          load_tile4<DP>(&maps.q, q_full, sQ, 0, it.head, it.q0);
+          ++qn;
+        }
+        for (int t = it.kt0; ok && t < it.kt1; ++t, ++kn) {
+          const int s = kn % NS;
+          const uint32_t ph = ((kn / NS) & 1) ^ 1;
+          ok = mbar_wait(&k_empty[s], ph, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 2));
+          if (!ok) break;
+          mbar_arrive_expect_tx(&k_full[s], C::kTile);
+          load_tile4<DP>(&maps.k, &k_full[s], sK + s * C::kTile, it.head, it.k0 + t * kTileRows, it.kb);
+          if (BIAS) {
+            ok = mbar_wait(b_empty, (bn & 1) ^ 1, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 3));
+            if (ok) {
+              mbar_arrive_expect_tx(b_full, 2 * kBlk);
+              for (int h = 0; h < 2; ++h)
+                tma_load_4d(&maps.bias, b_full, sB + h * kBlk, t * kTileRows + h * 64, it.pos0, it.head,
+                            it.seq / a.bias_seqs);
+              ++bn;
+            }
+          }
+          ok = ok && mbar_wait(&v_empty[s], ph, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 4));
+          if (!ok) {
+            mbar_wait_drain(&k_full[s], (kn / NS) & 1);   // issued alone: not seen by the drain below
+            break;
+          }
+          mbar_arrive_expect_tx(&v_full[s], C::kTile);
+          load_tile4<DP>(&maps.v, &v_full[s], sV + s * C::kTile, it.head, it.k0 + t * kTileRows, it.kb);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    }
+    if (lane == 0) {   // copies in flight land before the block may exit
+      if (qn) mbar_wait_drain(q_full, (qn - 1) & 1);
+      for (int i = kn > NS ? kn - NS : 0; i < kn; ++i) {
+        mbar_wait_drain(&k_full[i % NS], (i / NS) & 1);
+        mbar_wait_drain(&v_full[i % NS], (i / NS) & 1);
+      }
+      if (bn) mbar_wait_drain(b_full, (bn - 1) & 1);
+    }
+  } else if (warp == 5) {
+    // ------------------------------------------------------------------------ MMA
+    constexpr uint32_t id_s = idesc_f16(IsBf16<T>::v, 128, 128, 0, 0);
+    constexpr uint32_t id_o = idesc_f16(IsBf16<T>::v, 128, DP, 0, 1);
+    const uint32_t q_addr = smem_u32(sQ);
+    int qn = 0, kn = 0;        // items with keys; key tiles
+    bool ok = true;
+    while (ok && walk.next(a, it)) {
+      const int n = it.kt1 - it.kt0;
+      if (n <= 0) continue;
+      ok = mbar_wait_warp(q_full, qn & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 1));
+      for (int j = 0; ok && j <= n; ++j) {
+        // scores of tile j are issued behind P V of tile j - 1: the tensor pipe runs them
+        // in order, so S may overwrite the P that P V reads
+        if (j > 0) {
+          const int kj = kn + j - 1, s = kj % NS;
+          const int kt = it.kt0 + j - 1;
+          uint32_t keep[4];
+          if (a.key_mask) key_bits(a, it, kt, lane, keep);
+          ok = mbar_wait_warp(&v_full[s], (kj / NS) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 2));
+          if (!ok) break;
+          const int valid = it.klen - kt * kTileRows;
+          if (a.key_mask) {
+            if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
+              zero_rows_masked<DP>(sV + s * C::kTile, keep, lane);
+              fence_proxy_async_smem();
+              __syncwarp();
+            }
+          } else if (valid < kTileRows) {
+            zero_rows_from<DP>(sV + s * C::kTile, valid, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          ok = mbar_wait_warp(p_ready, kj & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 3));
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            mma_cols(tmem + 128, tmem, smem_u32(sV + s * C::kTile), id_o, j > 1);
+            umma_commit(&v_empty[s]);
+            if (j == n) umma_commit(o_full);
+          }
+          __syncwarp();
+        }
+        if (j < n) {
+          const int kj = kn + j, s = kj % NS;
+          ok = mbar_wait_warp(&k_full[s], (kj / NS) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 4));
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            mma_rows(tmem, q_addr, smem_u32(sK + s * C::kTile), id_s, a.ksteps);
+            umma_commit(s_full);
+            umma_commit(&k_empty[s]);
+            if (j == n - 1) umma_commit(q_empty);
+          }
+          __syncwarp();
+        }
+      }
+      kn += n;
+      ++qn;
+    }
+    if (lane == 0) {
+      umma_commit(drain);
+      mbar_wait_drain(drain, 0);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax, epilogue
+    const int row = threadIdx.x;
+    const int tok = row / a.group, gi = row - tok * a.group;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const float c = BIAS ? kLog2e : a.scale * kLog2e;     // scores to powers of two
+    int kn = 0, on = 0;
+    T* out = static_cast<T*>(a.out);
+    if (a.walk == WALK_LIST) {
+      // rows of no sequence: in front of the first, behind the last
+      const int lo = min(max(a.cu_q[0], 0), a.q_rows), hi = min(max(a.cu_q[a.seqs], lo), a.q_rows);
+      const long long per = static_cast<long long>(a.heads) * a.dim / 8;
+      const long long gone = (static_cast<long long>(lo) + a.q_rows - hi) * per;
+      for (long long i = static_cast<long long>(blockIdx.x) * 128 + row; i < gone;
+           i += static_cast<long long>(gridDim.x) * 128)
+        reinterpret_cast<uint4*>(out)[i < lo * per ? i : hi * per + (i - lo * per)] = make_uint4(0, 0, 0, 0);
+    }
+    bool ok = true;
+    while (ok && walk.next(a, it)) {
+      const bool live = tok < it.nq && row < a.group * a.tq;
+      const int seen = a.causal ? min(it.klen, it.pos0 + tok + it.off + 1) : it.klen;
+      float m = -INFINITY, l = 0.f;
+      for (int kt = it.kt0; kt < it.kt1; ++kt, ++kn) {
+        uint32_t keep[4];
+        const int lim = seen - kt * kTileRows;
+        bool cut = lim < kTileRows;
+        if (a.key_mask) {
+          key_bits(a, it, kt, lane, keep);
+          cut = cut || (keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu;
+        } else {
+          keep[0] = keep[1] = keep[2] = keep[3] = 0xffffffffu;
+        }
+        cut = __any_sync(0xffffffffu, cut);
+        if (BIAS) {
+          ok = mbar_wait_warp(b_full, kn & 1, a.err, err_code(KERNEL_ATTN, ROLE_EPILOGUE, 1));
+          if (!ok) break;
+        }
+        ok = mbar_wait_warp(s_full, kn & 1, a.err, err_code(KERNEL_ATTN, ROLE_EPILOGUE, 2));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t r[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) FTM_TMEM_LD32_NOWAIT(lanes + q * 32, r[q]);
+        tmem_wait_ld();
+        if (BIAS) {
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            float f[8];
+            unpack8(*reinterpret_cast<const uint4*>(sB + (q >> 3) * kBlk + sw128_off(row, q & 7)),
+                    IsBf16<T>::v, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              uint32_t& x = r[q >> 2][(q & 3) * 8 + e];
+              x = __float_as_uint(fmaf(__uint_as_float(x), a.scale, f[e]));
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(b_empty);
+        }
+        if (cut) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t on_bits = keep[q] & bits_below(lim, q);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((on_bits >> e) & 1u)) r[q][e] = 0xff800000u;   // -inf
+          }
+        }
+        float top[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) top[q] = fmaxf(top[q], __uint_as_float(r[q][e]));
+        const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        // keep the old maximum as the reference while it is within 2^8 of the new one
+        const bool grow = (mt - m) * c > 8.f || (m == -INFINITY && mt > m);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float f = grow ? (m == -INFINITY ? 0.f : ex2((m - mt) * c)) : 1.f;
+          if (grow) {
+            m = mt;
+            l *= f;
+          }
+          if (kt > it.kt0) {
+#pragma unroll
+            for (int q = 0; q < DP / 32; ++q) {
+              uint32_t o[32];
+              FTM_TMEM_LD32_NOWAIT(lanes + 128 + q * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(lanes + 128 + q * 32, o);
+            }
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        const float nref = BIAS ? ref : -ref * c;
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int i = q * 64 + 2 * e;
+            float2 x = make_float2(__uint_as_float(r[i >> 5][i & 31]), __uint_as_float(r[i >> 5][(i & 31) + 1]));
+            if (BIAS) {   // the difference first: scores near the type's lowest value stay exact
+              x = make_float2((x.x - nref) * c, (x.y - nref) * c);
+            } else {
+              x = __ffma2_rn(x, make_float2(c, c), make_float2(nref, nref));
+            }
+            const float2 p = make_float2(ex2(x.x), ex2(x.y));
+            sum[e & 1] = __fadd2_rn(sum[e & 1], p);
+            pk[e] = pack16<T>(p.x, p.y);
+          }
+          tmem_st32(lanes + q * 32, pk);
+        }
+        l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready);
+      }
+      if (!ok) break;
+      const bool any = it.kt1 > it.kt0;
+      if (any) {
+        ok = mbar_wait_warp(o_full, on & 1, a.err, err_code(KERNEL_ATTN, ROLE_EPILOGUE, 3));
+        if (!ok) break;
+        ++on;
+        tc_fence_after();
+      }
+      const int head = it.head * a.group + gi;
+      const size_t orow = (static_cast<size_t>(it.q0) + tok) * a.heads + head;
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+      for (int q = 0; q < DP / 32; ++q) {
+        uint32_t o[32];
+        if (any) {
+          FTM_TMEM_LD32_NOWAIT(lanes + 128 + q * 32, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+        }
+        if (!live) continue;
+        if (it.slot >= 0) {
+          float* po = a.part_o + (static_cast<size_t>(it.slot) * a.group + gi) * DP + q * 32;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            reinterpret_cast<uint4*>(po)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (q * 32 + e * 8 >= a.dim) break;
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(o[e * 8 + k]) * inv;
+            *reinterpret_cast<uint4*>(out + orow * a.dim + q * 32 + e * 8) =
+                make_uint4(pack16<T>(f[0], f[1]), pack16<T>(f[2], f[3]), pack16<T>(f[4], f[5]),
+                           pack16<T>(f[6], f[7]));
+          }
+        }
+      }
+      if (live && it.slot >= 0) a.part_ml[static_cast<size_t>(it.slot) * a.group + gi] = make_float2(m, l);
+      if (live && a.stats)   // a row without keys: p = 2^-inf = 0 in the backward
+        a.stats[orow] = l > 0.f || l != l ? make_float2(m, __log2f(l)) : make_float2(0.f, INFINITY);
+      tc_fence_before();   // O read before the next item's first P V is released by p_ready
+    }
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 5) tmem_dealloc(tmem, 256);
+}
+
+// Joins the partial results of a cache walk: block (sequence, head) x query head of the group.
+// A (sequence, head) whose tiles lie in one block of the walk was written by it.
+template <int DP, typename T>
+__global__ void __launch_bounds__(DP)
+attn_combine_kernel(const __grid_constant__ AttnArgs a, int blocks) {
+  grid_dep_wait();
+  const int seq = blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads, gi = blockIdx.y;
+  __shared__ int red[2][DP / 32];
+  int before = 0, all = 0;
+  for (int i = threadIdx.x; i < a.seqs; i += DP) {
+    const int n = (cache_len(a, i) + kTileRows - 1) / kTileRows;
+    all += n;
+    if (i < seq) before += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    red[0][threadIdx.x >> 5] = before;
+    red[1][threadIdx.x >> 5] = all;
+  }
+  __syncthreads();
+  before = all = 0;
+  for (int w = 0; w < DP / 32; ++w) {
+    before += red[0][w];
+    all += red[1][w];
+  }
+  const int tiles = (cache_len(a, seq) + kTileRows - 1) / kTileRows;
+  const int per = cache_per_block(all * a.kv_heads, blocks);
+  const int d = threadIdx.x;
+  const size_t orow = (static_cast<size_t>(seq) * a.heads + head * a.group + gi) * a.dim + d;
+  T* out = static_cast<T*>(a.out);
+  if (tiles == 0) {          // no keys: zeros
+    if (d < a.dim) out[orow] = T(0.f);
+    return;
+  }
+  const int t0 = before * a.kv_heads + head * tiles, t1 = t0 + tiles;
+  const int c0 = t0 / per, c1 = (t1 - 1) / per;
+  if (c0 == c1) return;
+  const float c = a.scale * kLog2e;
+  float m = -INFINITY;
+  for (int b = c0; b <= c1; ++b) {
+    const int slot = 2 * b + (b == c0 && t0 != b * per ? 1 : 0);
+    m = fmaxf(m, a.part_ml[static_cast<size_t>(slot) * a.group + gi].x);
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o = 0.f;
+#pragma unroll 4
+  for (int b = c0; b <= c1; ++b) {
+    const int slot = 2 * b + (b == c0 && t0 != b * per ? 1 : 0);
+    const size_t i = static_cast<size_t>(slot) * a.group + gi;
+    const float2 ml = a.part_ml[i];
+    const float f = ml.x == -INFINITY && ml.y == 0.f ? 0.f : ex2((ml.x - ref) * c);
+    l = fmaf(ml.y, f, l);
+    o = fmaf(a.part_o[i * DP + d], f, o);
+  }
+  if (d < a.dim) out[orow] = T(l > 0.f || l != l ? o / l : 0.f);
+}
+
+// Lists of a packed batch's tiles, (sequence, tile), by descending number of tiles of the
+// other side they meet: block 0 the query tiles, block 1 the key tiles. A counting sort
+// over that number; the order within equal ones varies and changes no result.
+__global__ void __launch_bounds__(1024)
+attn_lists_kernel(const __grid_constant__ AttnArgs a, int2* q_list, int q_cap, int2* k_list, int k_cap,
+                  int* counts) {
+  constexpr int kBuckets = 1024;
+  __shared__ int hist[kBuckets], warp_sum[32];
+  const bool kv = blockIdx.x == 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  hist[threadIdx.x] = 0;
+  grid_dep_wait();
+  __syncthreads();
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int s = warp; s < a.seqs; s += 32) {
+      int q0, qn, k0, kn;
+      seq_range(a.cu_q, s, 0, a.q_rows, q0, qn);
+      seq_range(a.cu_k, s, 0, a.kv_rows, k0, kn);
+      const int tiles = kv ? (kn + kTileRows - 1) / kTileRows : (qn + a.tq - 1) / a.tq;
+      for (int t = lane; t < tiles; t += 32) {
+        Item it;
+        if (kv) kv_item(a, s, t, 0, it);
+        else q_item(a, s, t, 0, it);
+        const int cost = min(kBuckets - 1, it.kt1 - it.kt0);
+        const int at = atomicAdd(&hist[kBuckets - 1 - cost], 1);
+        if (pass == 1 && at < (kv ? k_cap : q_cap)) (kv ? k_list : q_list)[at] = make_int2(s, t);
+      }
+    }
+    __syncthreads();
+    if (pass == 0) {     // counts -> first places
+      const int n = hist[threadIdx.x];
+      int inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (lane == 31) warp_sum[warp] = inc;
+      __syncthreads();
+      if (warp == 0) {
+        int w = warp_sum[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, w, o);
+          if (lane >= o) w += v;
+        }
+        warp_sum[lane] = w;
+      }
+      __syncthreads();
+      const int end = inc + (warp ? warp_sum[warp - 1] : 0);
+      hist[threadIdx.x] = end - n;
+      if (threadIdx.x == kBuckets - 1) counts[kv ? 1 : 0] = min(end, kv ? k_cap : q_cap);
+      __syncthreads();
+    }
+  }
+  grid_dep_release();
+}
+
+template <int DP, bool BIAS, typename T>
+cudaError_t go_fwd(const AttnLaunch& l) {
+  auto kern = attn_fwd_kernel<DP, BIAS, T>;
+  using C = FwdCfg<DP, BIAS>;
+  const cudaError_t e = set_smem_once(reinterpret_cast<const void*>(kern), C::kSmem);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kern, dim3(attn_fwd_grid(l)), dim3(kFwdThreads), C::kSmem, l.stream, nullptr, 0, l.m,
+                    l.a);
+}
+
+template <bool BIAS>
+cudaError_t go_fwd_dp(const AttnLaunch& l) {
+  if (l.dp == 64) return l.bf16 ? go_fwd<64, BIAS, __nv_bfloat16>(l) : go_fwd<64, BIAS, __half>(l);
+  return l.bf16 ? go_fwd<128, BIAS, __nv_bfloat16>(l) : go_fwd<128, BIAS, __half>(l);
+}
+
+}  // namespace
+
+// Two blocks per SM (one with a bias at DP = 128, whose shared memory allows no second), never
+// more than there are items: an item of the list per head, or a key tile of the cache.
+int attn_fwd_grid(const AttnLaunch& l) {
+  const AttnArgs& a = l.a;
+  const long long slots = static_cast<long long>(l.sms) * ((l.bias && l.dp == 128) ? 1 : 2);
+  long long items;
+  if (a.walk == WALK_LIST)
+    items = (static_cast<long long>(a.q_rows + a.tq - 1) / a.tq + a.seqs) * a.kv_heads;
+  else if (a.walk == WALK_UNIFORM)
+    items = static_cast<long long>(a.seqs) * a.q_tiles * a.kv_heads;
+  else
+    items = static_cast<long long>(a.seqs) * a.kv_heads * ((a.kv_rows + kTileRows - 1) / kTileRows);
+  return static_cast<int>(items < slots ? (items > 0 ? items : 1) : slots);
+}
+
+cudaError_t launch_attn_fwd(const AttnLaunch& l) { return l.bias ? go_fwd_dp<true>(l) : go_fwd_dp<false>(l); }
+
+cudaError_t launch_attn_combine(const AttnLaunch& l, int grid_fwd) {
+  const dim3 grid(l.a.seqs * l.a.kv_heads, l.a.group);
+  if (l.dp == 64)
+    return l.bf16 ? launch_pdl(attn_combine_kernel<64, __nv_bfloat16>, grid, dim3(64), 0, l.stream, nullptr, 0, l.a, grid_fwd)
+                  : launch_pdl(attn_combine_kernel<64, __half>, grid, dim3(64), 0, l.stream, nullptr, 0, l.a, grid_fwd);
+  return l.bf16 ? launch_pdl(attn_combine_kernel<128, __nv_bfloat16>, grid, dim3(128), 0, l.stream, nullptr, 0, l.a, grid_fwd)
+                : launch_pdl(attn_combine_kernel<128, __half>, grid, dim3(128), 0, l.stream, nullptr, 0, l.a, grid_fwd);
+}
+
+cudaError_t launch_attn_lists(const AttnLaunch& l, int2* q_list, int q_cap, int2* k_list, int k_cap,
+                              int* counts) {
+  return launch_pdl(attn_lists_kernel, dim3(k_list ? 2 : 1), dim3(1024), 0, l.stream, nullptr, 0, l.a, q_list,
+                    q_cap, k_list, k_cap, counts);
+}
+
+}  // namespace ftm

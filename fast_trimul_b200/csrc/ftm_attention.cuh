@@ -1,0 +1,279 @@
+// Shared pieces of the attention kernels (forward and backward): the problem as the
+// kernels see it, the walk over its tiles, and the tcgen05 forms they need beside
+// ftm_common.cuh's.
+//
+// A tile of queries is up to 128 rows of one key / value head: row = token * G + g over
+// the G query heads that share the head, so grouped heads read K and V once, and one new
+// token of a sequence still fills G rows. A tile of keys is 128 positions. Head
+// dimensions are padded to DP = 64 or 128 in shared memory by the zero fill of TMA.
+#pragma once
+
+#include "ftm_kernels.h"
+
+namespace ftm {
+
+constexpr int kTileRows = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// how the items of a launch are numbered
+enum : int { WALK_LIST = 0, WALK_UNIFORM = 1, WALK_CACHE = 2 };
+
+struct AttnArgs {
+  int heads, kv_heads, group, dim;
+  int tq;                    // tokens per query tile: 128 / group
+  int ksteps;                // 16-element steps of the head dimension
+  int seqs, q_rows, kv_rows; // kv_rows: rows of one batch entry of a cache
+  int q_len, k_len;          // every sequence's, where cu_q is null
+  int walk;
+  int q_tiles, k_tiles;      // per sequence (uniform walk)
+  int causal;
+  float scale;
+  const int* cu_q;           // seqs + 1 first rows, on the device; null: uniform
+  const int* cu_k;
+  const int* k_lens;         // cache walk: keys of each sequence
+  const int2* list;          // list walk: (sequence, tile), longest first
+  const int* count;          // entries of the list
+  const uint8_t* key_mask;   // one byte per key row, 0: not seen; may be null
+  int bias_seqs;             // consecutive sequences that share a bias
+  int splits;                // bias gradient: parts of those sequences
+  // outputs and operands that are read by plain loads; contiguous unless strides follow
+  void* out;
+  const void* o;             // forward output (backward)
+  const void* g;             // its gradient: strides in elements
+  long long g_row, g_head;
+  float2* stats;             // (row maximum m, log2 of the row sum) per (row, head)
+  float4* bstats;            // backward: (see attn_delta_kernel)
+  float* part_o;             // cache walk: partial results of split sequences
+  float2* part_ml;
+  void* dq;
+  void* dk;
+  void* dv;
+  void* dbias;
+  float* dbias_part;
+  int* err;
+};
+
+struct Item {
+  int seq, head;      // sequence, key / value head
+  int q0, nq;         // first global token row of the query tile, its tokens
+  int pos0;           // position of that token in its sequence
+  int k0, klen;       // first key row, keys of the sequence
+  int kb;             // batch coordinate of the key maps
+  int off;            // query i sees keys j <= i + off (causal)
+  int kt0, kt1;       // tiles of keys (or of queries, in the kv walk)
+  int slot;           // partial result, -1: none
+  int tile;
+};
+
+__device__ __forceinline__ void seq_range(const int* cu, int i, int len, int rows, int& s, int& n) {
+  if (cu) {   // clamped: whatever the array holds, no row outside the tensors is touched
+    s = min(max(cu[i], 0), rows);
+    n = min(max(cu[i + 1], s), rows) - s;
+  } else {
+    s = i * len;
+    n = len;
+  }
+}
+
+__device__ __forceinline__ int cache_len(const AttnArgs& a, int i) {
+  return min(max(a.k_lens[i], 0), a.kv_rows);
+}
+
+// the query tile `tile` of sequence `seq` and head `head`, with the tiles of keys it sees
+__device__ __forceinline__ void q_item(const AttnArgs& a, int seq, int tile, int head, Item& it) {
+  int qs, qn;
+  seq_range(a.cu_q, seq, a.q_len, a.q_rows, qs, qn);
+  if (a.k_lens) {
+    it.k0 = 0;
+    it.klen = cache_len(a, seq);
+    it.kb = seq;
+  } else {
+    seq_range(a.cu_k, seq, a.k_len, a.kv_rows, it.k0, it.klen);
+    it.kb = 0;
+  }
+  it.seq = seq;
+  it.head = head;
+  it.tile = tile;
+  it.pos0 = tile * a.tq;
+  it.q0 = qs + it.pos0;
+  it.nq = min(a.tq, qn - it.pos0);
+  it.off = it.klen - qn;
+  int seen = it.klen;
+  if (a.causal) seen = max(0, min(seen, it.pos0 + it.nq + it.off));
+  it.kt0 = 0;
+  it.kt1 = (seen + kTileRows - 1) / kTileRows;
+  it.slot = -1;
+}
+
+// the key tile `tile`, with the query tiles that see it
+__device__ __forceinline__ void kv_item(const AttnArgs& a, int seq, int tile, int head, Item& it) {
+  int qs, qn;
+  seq_range(a.cu_q, seq, a.q_len, a.q_rows, qs, qn);
+  seq_range(a.cu_k, seq, a.k_len, a.kv_rows, it.k0, it.klen);
+  it.kb = 0;
+  it.seq = seq;
+  it.head = head;
+  it.tile = tile;
+  it.q0 = qs;
+  it.nq = qn;
+  it.pos0 = 0;
+  it.off = it.klen - qn;
+  it.kt1 = (qn + a.tq - 1) / a.tq;
+  it.kt0 = a.causal ? min(it.kt1, max(0, tile * kTileRows - it.off) / a.tq) : 0;
+  it.slot = -1;
+}
+
+template <bool KV>
+__device__ __forceinline__ bool walk_item(const AttnArgs& a, int n, Item& it) {
+  if (a.walk == WALK_LIST) {
+    const int w = n / a.kv_heads;
+    if (w >= *a.count) return false;
+    const int2 e = a.list[w];
+    if (KV) kv_item(a, e.x, e.y, n % a.kv_heads, it);
+    else q_item(a, e.x, e.y, n % a.kv_heads, it);
+    return true;
+  }
+  const int tiles = KV ? a.k_tiles : a.q_tiles;
+  const int rest = n / tiles;
+  if (rest >= a.seqs * a.kv_heads) return false;
+  if (KV) kv_item(a, rest / a.kv_heads, n % tiles, rest % a.kv_heads, it);
+  else q_item(a, rest / a.kv_heads, n % tiles, rest % a.kv_heads, it);
+  return true;
+}
+
+// ------------------------------------------------------------------- tcgen05 forms
+// D (+)= A[tmem] * B[smem desc]; A: 16-bit pairs, 8 columns per 16-element step
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+      "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack16<__half>(float a, float b) { return pack_half2(a, b); }
+template <>
+__device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float a, float b) { return pack_bf162(a, b); }
+
+template <typename T>
+struct IsBf16 { static constexpr int v = 0; };
+template <>
+struct IsBf16<__nv_bfloat16> { static constexpr int v = 1; };
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---------------------------------------------------------------------- MMA shapes
+// Tiles in shared memory: DP / 64 blocks of 128 rows x 128 bytes (128-byte swizzle).
+constexpr int kBlk = kTileRows * 128;   // bytes of one 64-element block
+
+// D[128 x 128] = A[128 rows x dim] B[128 rows x dim]^T, both K-major
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int ksteps) {
+  for (int k = 0; k < ksteps; ++k) {
+    const uint32_t o = (k >> 2) * kBlk + (k & 3) * 32;
+    umma_f16(d, kmajor_desc(a + o), kmajor_desc(b + o), idesc, k > 0 ? 1u : 0u);
+  }
+}
+// D[128 x DP] (+)= A[tmem, 128 x 128] B[128 rows x DP], B MN-major
+__device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t idesc,
+                                         bool accumulate) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    umma_f16_ts(d, a_tmem + k * 8, sw128_desc(b + k * 2048, kBlk, 1024), idesc,
+                (accumulate || k > 0) ? 1u : 0u);
+}
+
+template <int DP>
+__device__ __forceinline__ void load_tile4(const CUtensorMap* map, uint64_t* bar, uint8_t* dst, int c1,
+                                           int c2, int c3) {
+#pragma unroll
+  for (int h = 0; h < DP / 64; ++h) tma_load_4d(map, bar, dst + h * kBlk, h * 64, c1, c2, c3);
+}
+
+// Rows [first, 128) of a tile set to zero by one warp: rows behind a sequence's end belong
+// to somebody else, and a zero weight times what they hold need not be zero.
+template <int DP>
+__device__ __forceinline__ void zero_rows_from(uint8_t* tile, int first, int lane) {
+  for (int h = 0; h < DP / 64; ++h)
+    for (int i = first * 8 + lane; i < kTileRows * 8; i += 32)
+      reinterpret_cast<uint4*>(tile + h * kBlk)[i] = make_uint4(0, 0, 0, 0);
+}
+// the same for the rows whose bit is clear
+template <int DP>
+__device__ __forceinline__ void zero_rows_masked(uint8_t* tile, const uint32_t (&keep)[4], int lane) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    for (uint32_t gone = ~keep[w]; gone; gone &= gone - 1) {
+      const int r = w * 32 + __ffs(gone) - 1;
+      if (lane < DP / 8)
+        *reinterpret_cast<uint4*>(tile + (lane >> 3) * kBlk + r * 128 + (lane & 7) * 16) =
+            make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+// bits of the keys of a tile that exist and are not masked (the same in every lane)
+__device__ __forceinline__ void key_bits(const AttnArgs& a, const Item& it, int kt, int lane,
+                                         uint32_t (&w)[4]) {
+  const int c0 = kt * kTileRows;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = c0 + i * 32 + lane;
+    bool on = c < it.klen;
+    if (on && a.key_mask) on = a.key_mask[static_cast<size_t>(it.k0) + c] != 0;
+    w[i] = __ballot_sync(0xffffffffu, on);
+  }
+}
+
+// bits [0, lim) of a 128-bit row
+__device__ __forceinline__ uint32_t bits_below(int lim, int word) {
+  const int n = lim - word * 32;
+  return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+}
+
+struct AttnMaps {
+  CUtensorMap q, k, v, g, bias;
+};
+
+// host side ------------------------------------------------------------------------
+struct AttnLaunch {
+  AttnArgs a;
+  AttnMaps m;
+  int dp, bf16, bias, sms;
+  cudaStream_t stream;
+};
+cudaError_t launch_attn_fwd(const AttnLaunch& l);
+cudaError_t launch_attn_combine(const AttnLaunch& l, int grid_fwd);
+cudaError_t launch_attn_lists(const AttnLaunch& l, int2* q_list, int q_cap, int2* k_list, int k_cap,
+                              int* counts);
+cudaError_t launch_attn_delta(const AttnLaunch& l);
+cudaError_t launch_attn_dq(const AttnLaunch& l);
+cudaError_t launch_attn_dkv(const AttnLaunch& l);
+cudaError_t launch_attn_dbias(const AttnLaunch& l);
+int attn_fwd_grid(const AttnLaunch& l);
+
+}  // namespace ftm

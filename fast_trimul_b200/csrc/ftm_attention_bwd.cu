@@ -1,0 +1,999 @@
+// Attention backward (sm_100a). With p the forward's weights, recomputed tile by tile from the
+// row maximum and sum it kept, g the output's gradient and d = rowsum(g * o):
+//
+//   dv = p^T g,   dp = g v^T,   ds = p (dp - d),   dq = scale ds k,   dk = scale ds^T q,
+//   dbias = sum over the rows that share it of ds.
+//
+// Three kernels on the same scheme -- two products into TMEM, the elementwise part in
+// registers, a 16-bit operand back into TMEM for the accumulating products:
+//   dq     one query tile, loop over its key tiles:    S, dP -> dS;   dQ += dS K
+//   dkv    one key tile, loop over its query tiles:    S^T, dP^T -> P^T, dS^T;
+//          dV += P^T dO, dK += dS^T Q; with grouped heads the loop covers the whole group
+//   dbias  one tile of the bias, loop over the rows that share it, sums in registers
+// Each result has one owner, so there are no atomics and a call gives the same bits every
+// time, at the price of forming S and dP twice (7 products instead of 5). fp32 everywhere
+// but the 16-bit operands P and dS, rounded once like the inputs of any product here.
+//
+// Roles: warps 0-7 elementwise (two per TMEM lane quarter, each half of the columns), warp 8
+// TMA (and, in dkv, the per-query constants), warp 9 MMA. All 512 TMEM columns, one block
+// per SM: dq holds S twice (the next tile's scores are formed under this one's
+// elementwise part), dkv holds S^T, dP^T, dV, dK.
+#include "ftm_attention.cuh"
+
+namespace ftm {
+namespace {
+
+enum : int { KERNEL_DQ = 5, KERNEL_DKV = 6, KERNEL_DBIAS = 7 };
+constexpr int kBwdThreads = 320;
+
+// bstats of a (row, head): without a bias x = m c + log2(l) with c = scale log2(e), so that
+// p = 2^(c s - x); with one x = m, y = log2(l), p = 2^((t - x) log2(e) - y), which stays
+// exact for scores near the type's lowest value. z = rowsum(g * o). A row without keys has
+// log2(l) = inf, hence p = 0.
+template <typename T>
+__global__ void __launch_bounds__(256)
+attn_delta_kernel(const __grid_constant__ AttnArgs a, int lanes, int bias) {
+  grid_dep_wait();
+  const long long n = static_cast<long long>(a.q_rows) * a.heads;
+  const int per = blockDim.x / lanes, l = threadIdx.x % lanes;
+  const float c = a.scale * kLog2e;
+  // the bound is the same for all threads of a warp: the sums below exchange lanes
+  for (long long i0 = static_cast<long long>(blockIdx.x) * per; i0 < n; i0 += static_cast<long long>(gridDim.x) * per) {
+    const long long i = i0 + threadIdx.x / lanes;
+    float s = 0.f;
+    if (i < n && l * 8 < a.dim) {
+      const long long row = i / a.heads;
+      const int head = static_cast<int>(i - row * a.heads);
+      float x[8], y[8];
+      unpack8(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.o) + i * a.dim + l * 8), IsBf16<T>::v, x);
+      unpack8(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.g) + row * a.g_row + head * a.g_head + l * 8),
+              IsBf16<T>::v, y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s = fmaf(x[k], y[k], s);
+    }
+    for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (i < n && l == 0) {
+      const float2 st = a.stats[i];
+      a.bstats[i] = bias ? make_float4(st.x, st.y, s, 0.f) : make_float4(fmaf(st.x, c, st.y), 0.f, s, 0.f);
+    }
+  }
+  grid_dep_release();
+}
+
+// rows of no sequence, in front of the first and behind the last, set to zero
+template <typename T>
+__device__ __forceinline__ void zero_outside(const int* cu, int seqs, int rows, long long per, T* out, int t,
+                                             int threads) {
+  const int lo = min(max(cu[0], 0), rows), hi = min(max(cu[seqs], lo), rows);
+  const long long gone = (static_cast<long long>(lo) + rows - hi) * per;
+  for (long long i = static_cast<long long>(blockIdx.x) * threads + t; i < gone;
+       i += static_cast<long long>(gridDim.x) * threads)
+    reinterpret_cast<uint4*>(out)[i < lo * per ? i : hi * per + (i - lo * per)] = make_uint4(0, 0, 0, 0);
+}
+
+// COLS columns of an accumulator row, times f, as 16-bit values to out[0 .. dim)
+template <int COLS, typename T>
+__device__ __forceinline__ void store_acc(uint32_t taddr, int col0, int dim, float f, bool live, bool any, T* out) {
+#pragma unroll
+  for (int q = 0; q < COLS / 32; ++q) {
+    uint32_t o[32];
+    if (any) {
+      FTM_TMEM_LD32_NOWAIT(taddr + col0 + q * 32, o);
+      tmem_wait_ld();
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = 0;
+    }
+    if (!live) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = col0 + q * 32 + e * 8;
+      if (c >= dim) break;
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(o[e * 8 + k]) * f;
+      *reinterpret_cast<uint4*>(out + c) =
+          make_uint4(pack16<T>(x[0], x[1]), pack16<T>(x[2], x[3]), pack16<T>(x[4], x[5]), pack16<T>(x[6], x[7]));
+    }
+  }
+}
+
+// --------------------------------------------------------------------------------- dq
+template <int DP, bool BIAS>
+struct DqCfg {
+  static constexpr int kTile = DP / 64 * kBlk;
+  static constexpr int kOffG = kTile;
+  static constexpr int kOffK = 2 * kTile;
+  static constexpr int kOffV = 4 * kTile;
+  static constexpr int kOffB = 6 * kTile;
+  static constexpr int kOffBar = kOffB + (BIAS ? 2 * kBlk : 0);
+  static constexpr int kSmem = kOffBar + 256 + 1024;
+  static_assert(kSmem <= 232448, "dq exceeds 227 KB of shared memory");
+};
+
+template <int DP, bool BIAS, typename T>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnArgs a) {
+  using C = DqCfg<DP, BIAS>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sG = smem + C::kOffG;
+  uint8_t* sK = smem + C::kOffK;
+  uint8_t* sV = smem + C::kOffV;
+  uint8_t* sB = smem + C::kOffB;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* k_full = q_full + 2;
+  uint64_t* k_empty = q_full + 4;
+  uint64_t* v_full = q_full + 6;
+  uint64_t* v_empty = q_full + 8;
+  uint64_t* b_full = q_full + 10;
+  uint64_t* b_empty = q_full + 11;
+  uint64_t* s_full = q_full + 12;    // 2
+  uint64_t* dp_full = q_full + 14;
+  uint64_t* ds_ready = q_full + 15;
+  uint64_t* acc_full = q_full + 16;
+  uint64_t* drain = q_full + 17;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 18);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 18; ++i) mbar_init(q_full + i, i == 11 || i == 15 ? 8 : 1);
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dep_wait();
+  grid_dep_release();
+  // columns: S of even tiles 0, dP 128, dQ 256, S of odd tiles 384
+  int n = blockIdx.x;
+  Item it;
+
+  if (warp == 8) {
+    const uint32_t q_bytes = 2u * (DP / 64 * 128u * (a.group * a.tq));
+    int qn = 0, kn = 0;
+    bool ok = true;
+    for (; ok && walk_item<false>(a, n, it); n += gridDim.x) {
+      if (it.kt1 <= it.kt0) continue;
+      if (lane == 0) {
+        ok = mbar_wait(q_empty, (qn & 1) ^ 1, a.err, err_code(KERNEL_DQ, ROLE_PRODUCER, 1));
+        if (ok) {
+          mbar_arrive_expect_tx(q_full, q_bytes);
+          load_tile4<DP>(&maps.q, q_full, sQ, 0, it.head, it.q0);
+          load_tile4<DP>(&maps.g, q_full, sG, 0, it.head, it.q0);
+          ++qn;
+        }
+        for (int t = it.kt0; ok && t < it.kt1; ++t) {
+          const int s = kn & 1;
+          const uint32_t ph = ((kn >> 1) & 1) ^ 1;
+          ok = mbar_wait(&k_empty[s], ph, a.err, err_code(KERNEL_DQ, ROLE_PRODUCER, 2)) &&
+               mbar_wait(&v_empty[s], ph, a.err, err_code(KERNEL_DQ, ROLE_PRODUCER, 3)) &&
+               (!BIAS || mbar_wait(b_empty, (kn & 1) ^ 1, a.err, err_code(KERNEL_DQ, ROLE_PRODUCER, 4)));
+          if (!ok) break;
+          mbar_arrive_expect_tx(&k_full[s], C::kTile);
+          load_tile4<DP>(&maps.k, &k_full[s], sK + s * C::kTile, it.head, it.k0 + t * kTileRows, it.kb);
+          mbar_arrive_expect_tx(&v_full[s], C::kTile);
+          load_tile4<DP>(&maps.v, &v_full[s], sV + s * C::kTile, it.head, it.k0 + t * kTileRows, it.kb);
+          if (BIAS) {
+            mbar_arrive_expect_tx(b_full, 2 * kBlk);
+            for (int h = 0; h < 2; ++h)
+              tma_load_4d(&maps.bias, b_full, sB + h * kBlk, t * kTileRows + h * 64, it.pos0, it.head,
+                          it.seq / a.bias_seqs);
+          }
+          ++kn;
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    }
+    if (lane == 0) {
+      if (qn) mbar_wait_drain(q_full, (qn - 1) & 1);
+      for (int i = kn > 2 ? kn - 2 : 0; i < kn; ++i) {
+        mbar_wait_drain(&k_full[i & 1], (i >> 1) & 1);
+        mbar_wait_drain(&v_full[i & 1], (i >> 1) & 1);
+      }
+      if (BIAS && kn) mbar_wait_drain(b_full, (kn - 1) & 1);
+    }
+  } else if (warp == 9) {
+    constexpr uint32_t id_s = idesc_f16(IsBf16<T>::v, 128, 128, 0, 0);
+    constexpr uint32_t id_o = idesc_f16(IsBf16<T>::v, 128, DP, 0, 1);
+    const uint32_t q_addr = smem_u32(sQ), g_addr = smem_u32(sG);
+    int qn = 0, kn = 0;
+    bool ok = true;
+    // scores of key tile number i (of all this block meets); rows of K that are not keys of
+    // this sequence are cleared first, since 0 * K enters dQ
+    auto scores = [&](int i, int kt) -> bool {
+      const int s = i & 1;
+      uint32_t keep[4];
+      if (a.key_mask) key_bits(a, it, kt, lane, keep);
+      if (!mbar_wait_warp(&k_full[s], (i >> 1) & 1, a.err, err_code(KERNEL_DQ, ROLE_MMA, 2))) return false;
+      const int valid = it.klen - kt * kTileRows;
+      if (a.key_mask) {
+        if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
+          zero_rows_masked<DP>(sK + s * C::kTile, keep, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+      } else if (valid < kTileRows) {
+        zero_rows_from<DP>(sK + s * C::kTile, valid, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      tc_fence_after();
+      if (lane == 0) {
+        mma_rows(tmem + (s ? 384 : 0), q_addr, smem_u32(sK + s * C::kTile), id_s, a.ksteps);
+        umma_commit(&s_full[s]);
+      }
+      __syncwarp();
+      return true;
+    };
+    auto weights_grad = [&](int i) -> bool {
+      const int s = i & 1;
+      if (!mbar_wait_warp(&v_full[s], (i >> 1) & 1, a.err, err_code(KERNEL_DQ, ROLE_MMA, 3))) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        mma_rows(tmem + 128, g_addr, smem_u32(sV + s * C::kTile), id_s, a.ksteps);
+        umma_commit(dp_full);
+        umma_commit(&v_empty[s]);
+      }
+      __syncwarp();
+      return true;
+    };
+    for (; ok && walk_item<false>(a, n, it); n += gridDim.x) {
+      const int tiles = it.kt1 - it.kt0;
+      if (tiles <= 0) continue;
+      ok = mbar_wait_warp(q_full, qn & 1, a.err, err_code(KERNEL_DQ, ROLE_MMA, 1));
+      ok = ok && scores(kn, it.kt0) && weights_grad(kn);
+      for (int j = 0; ok && j < tiles; ++j, ++kn) {
+        if (j + 1 < tiles) ok = scores(kn + 1, it.kt0 + j + 1);
+        ok = ok && mbar_wait_warp(ds_ready, kn & 1, a.err, err_code(KERNEL_DQ, ROLE_MMA, 4));
+        if (ok && j + 1 < tiles) ok = weights_grad(kn + 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const int s = kn & 1;
+          mma_cols(tmem + 256, tmem + (s ? 384 : 0), smem_u32(sK + s * C::kTile), id_o, j > 0);
+          umma_commit(&k_empty[s]);
+          if (j + 1 == tiles) {
+            umma_commit(acc_full);
+            umma_commit(q_empty);
+          }
+        }
+        __syncwarp();
+      }
+      ++qn;
+    }
+    if (lane == 0) {
+      umma_commit(drain);
+      mbar_wait_drain(drain, 0);
+    }
+  } else {
+    const int quad = warp & 3, half = warp >> 2;
+    const int row = quad * 32 + lane;
+    const int tok = row / a.group, gi = row - tok * a.group;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const float c = a.scale * kLog2e;
+    T* dq = static_cast<T*>(a.dq);
+    if (a.walk == WALK_LIST)
+      zero_outside(a.cu_q, a.seqs, a.q_rows, static_cast<long long>(a.heads) * a.dim / 8, dq, threadIdx.x, 256);
+    int kn = 0, qn = 0;
+    bool ok = true;
+    for (; ok && walk_item<false>(a, n, it); n += gridDim.x) {
+      const bool live = tok < it.nq && row < a.group * a.tq;
+      const size_t orow = (static_cast<size_t>(it.q0) + tok) * a.heads + it.head * a.group + gi;
+      const int seen = a.causal ? min(it.klen, it.pos0 + tok + it.off + 1) : it.klen;
+      const float4 st = live ? a.bstats[orow] : make_float4(0.f, INFINITY, 0.f, 0.f);
+      const float ref = BIAS || live ? st.x : INFINITY;
+      for (int kt = it.kt0; kt < it.kt1; ++kt, ++kn) {
+        const int b = kn & 1;
+        const int lim = seen - kt * kTileRows;
+        uint32_t keep[4];
+        bool cut = lim < kTileRows;
+        if (a.key_mask) {
+          key_bits(a, it, kt, lane, keep);
+          cut = cut || (keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu;
+        } else {
+          keep[0] = keep[1] = keep[2] = keep[3] = 0xffffffffu;
+        }
+        cut = __any_sync(0xffffffffu, cut);
+        ok = mbar_wait_warp(&s_full[b], (kn >> 1) & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 1));
+        if (BIAS) ok = ok && mbar_wait_warp(b_full, kn & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 2));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t scol = lanes + (b ? 384 : 0);
+        uint32_t r[2][32];
+        FTM_TMEM_LD32_NOWAIT(scol + half * 64, r[0]);
+        FTM_TMEM_LD32_NOWAIT(scol + half * 64 + 32, r[1]);
+        tmem_wait_ld();
+        if (BIAS) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            float f[8];
+            unpack8(*reinterpret_cast<const uint4*>(sB + half * kBlk + sw128_off(row, q)), IsBf16<T>::v, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              uint32_t& x = r[q >> 2][(q & 3) * 8 + e];
+              x = __float_as_uint(fmaf(__uint_as_float(x), a.scale, f[e]));
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(b_empty);
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float x = __uint_as_float(r[q][e]);
+            r[q][e] = __float_as_uint(ex2(BIAS ? fmaf(x - ref, kLog2e, -st.y) : fmaf(x, c, -ref)));
+          }
+        if (cut) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const uint32_t on = keep[half * 2 + q] & bits_below(lim, half * 2 + q);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((on >> e) & 1u)) r[q][e] = 0u;
+          }
+        }
+        ok = mbar_wait_warp(dp_full, kn & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 3));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t pk[32];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t d[32];
+          FTM_TMEM_LD32_NOWAIT(lanes + 128 + half * 64 + q * 32, d);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float x0 = __uint_as_float(r[q][e]) * (__uint_as_float(d[e]) - st.z);
+            float x1 = __uint_as_float(r[q][e + 1]) * (__uint_as_float(d[e + 1]) - st.z);
+            if (cut) {   // a key that is not seen gives nothing, whatever its V holds
+              x0 = r[q][e] ? x0 : 0.f;
+              x1 = r[q][e + 1] ? x1 : 0.f;
+            }
+            pk[q * 16 + e / 2] = pack16<T>(x0, x1);
+          }
+        }
+        named_barrier_sync(1 + quad, 64);   // both halves have read S: dS goes over it
+        tmem_st32(scol + half * 32, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready);
+      }
+      if (!ok) break;
+      const bool any = it.kt1 > it.kt0;
+      if (any) {
+        ok = mbar_wait_warp(acc_full, qn & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 4));
+        if (!ok) break;
+        ++qn;
+        tc_fence_after();
+      }
+      store_acc<DP / 2>(lanes + 256, half * (DP / 2), a.dim, a.scale, live, any, dq + orow * a.dim);
+      tc_fence_before();
+    }
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// -------------------------------------------------------------------------------- dkv
+template <int DP, bool BIAS>
+struct DkvCfg {
+  static constexpr int kTile = DP / 64 * kBlk;
+  static constexpr int kOffV = kTile;
+  static constexpr int kOffQ = 2 * kTile;
+  static constexpr int kOffG = 4 * kTile;
+  static constexpr int kOffB = 6 * kTile;
+  static constexpr int kCols = (BIAS && DP == 128) ? 1 : 2;       // what shared memory leaves
+  static constexpr int kOffCol = kOffB + (BIAS ? 2 * kBlk : 0);   // kCols x 128 x (x, y, z)
+  static constexpr int kOffBar = kOffCol + kCols * kTileRows * 12;
+  static constexpr int kSmem = kOffBar + 256 + 1024;
+  static_assert(kSmem <= 232448, "dkv exceeds 227 KB of shared memory");
+};
+
+template <int DP, bool BIAS, typename T>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnArgs a) {
+  using C = DkvCfg<DP, BIAS>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sK = smem;
+  uint8_t* sV = smem + C::kOffV;
+  uint8_t* sQ = smem + C::kOffQ;
+  uint8_t* sG = smem + C::kOffG;
+  uint8_t* sB = smem + C::kOffB;
+  float* sC = reinterpret_cast<float*>(smem + C::kOffCol);   // [buffer][x: 128, y: 128, z: 128]
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* kv_empty = kv_full + 1;
+  uint64_t* q_full = kv_full + 2;
+  uint64_t* q_empty = kv_full + 4;
+  uint64_t* g_full = kv_full + 6;
+  uint64_t* g_empty = kv_full + 8;
+  uint64_t* b_full = kv_full + 10;
+  uint64_t* b_empty = kv_full + 11;
+  uint64_t* c_full = kv_full + 12;   // 2
+  uint64_t* c_empty = kv_full + 14;  // 2
+  uint64_t* s_full = kv_full + 16;
+  uint64_t* p_ready = kv_full + 17;
+  uint64_t* dp_full = kv_full + 18;
+  uint64_t* ds_ready = kv_full + 19;
+  uint64_t* acc_full = kv_full + 20;
+  uint64_t* drain = kv_full + 21;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_full + 22);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 22; ++i)
+      mbar_init(kv_full + i, i == 11 || i == 14 || i == 15 || i == 17 || i == 19 ? 8 : 1);
+    fence_mbar_init();
+  }
+  // rows of a query tile that no load writes (128 is no multiple of the group): zero once
+  {
+    const int used = a.group * a.tq;
+    if (used < kTileRows) {
+      for (int t = warp; t < 4; t += kBwdThreads / 32)
+        zero_rows_from<DP>(sQ + t * C::kTile, used, lane);
+      fence_proxy_async_smem();
+    }
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dep_wait();
+  grid_dep_release();
+  // columns: S^T / P^T 0, dP^T / dS^T 128, dV 256, dK 384
+  int n = blockIdx.x;
+  Item it;
+
+  if (warp == 8) {
+    const uint32_t q_bytes = DP / 64 * 128u * (a.group * a.tq);
+    int in = 0, qn = 0;
+    bool ok = true;
+    for (; ok && walk_item<true>(a, n, it); n += gridDim.x) {
+      if (it.kt1 <= it.kt0) continue;
+      ok = mbar_wait_warp(kv_empty, (in & 1) ^ 1, a.err, err_code(KERNEL_DKV, ROLE_PRODUCER, 1));
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(kv_full, 2 * C::kTile);
+        load_tile4<DP>(&maps.k, kv_full, sK, it.head, it.k0 + it.tile * kTileRows, 0);
+        load_tile4<DP>(&maps.v, kv_full, sV, it.head, it.k0 + it.tile * kTileRows, 0);
+      }
+      ++in;
+      for (int t = it.kt0; t < it.kt1; ++t) {
+        const int s = qn & 1;
+        const uint32_t ph = ((qn >> 1) & 1) ^ 1;
+        ok = mbar_wait_warp(&q_empty[s], ph, a.err, err_code(KERNEL_DKV, ROLE_PRODUCER, 2)) &&
+             mbar_wait_warp(&g_empty[s], ph, a.err, err_code(KERNEL_DKV, ROLE_PRODUCER, 3)) &&
+             (!BIAS || mbar_wait_warp(b_empty, (qn & 1) ^ 1, a.err, err_code(KERNEL_DKV, ROLE_PRODUCER, 4)));
+        if (!ok) break;
+        if (lane == 0) {
+          const int row = it.q0 + t * a.tq;
+          mbar_arrive_expect_tx(&q_full[s], q_bytes);
+          load_tile4<DP>(&maps.q, &q_full[s], sQ + s * C::kTile, 0, it.head, row);
+          mbar_arrive_expect_tx(&g_full[s], q_bytes);
+          load_tile4<DP>(&maps.g, &g_full[s], sG + s * C::kTile, 0, it.head, row);
+          if (BIAS) {
+            mbar_arrive_expect_tx(b_full, 2 * kBlk);
+            for (int h = 0; h < 2; ++h)
+              tma_load_4d(&maps.bias, b_full, sB + h * kBlk, it.tile * kTileRows + h * 64, t * a.tq, it.head,
+                          it.seq / a.bias_seqs);
+          }
+        }
+        ++qn;
+        __syncwarp();
+        // the constants of this tile's queries, one per column of S^T
+        const int cn = qn - 1, cb = cn % C::kCols;
+        ok = mbar_wait_warp(&c_empty[cb], ((cn / C::kCols) & 1) ^ 1, a.err, err_code(KERNEL_DKV, ROLE_PRODUCER, 5));
+        if (!ok) break;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int r = w * 32 + lane, tok = r / a.group;
+          const bool live = r < a.group * a.tq && t * a.tq + tok < it.nq;
+          float4 st = make_float4(BIAS ? 0.f : INFINITY, INFINITY, 0.f, 0.f);   // p = 0
+          if (live)
+            st = a.bstats[(static_cast<size_t>(it.q0) + t * a.tq + tok) * a.heads + it.head * a.group + r - tok * a.group];
+          sC[cb * 384 + r] = st.x;
+          sC[cb * 384 + 128 + r] = st.y;
+          sC[cb * 384 + 256 + r] = st.z;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c_full[cb]);
+      }
+    }
+    if (lane == 0) {
+      if (in) mbar_wait_drain(kv_full, (in - 1) & 1);
+      for (int i = qn > 2 ? qn - 2 : 0; i < qn; ++i) {
+        mbar_wait_drain(&q_full[i & 1], (i >> 1) & 1);
+        mbar_wait_drain(&g_full[i & 1], (i >> 1) & 1);
+      }
+      if (BIAS && qn) mbar_wait_drain(b_full, (qn - 1) & 1);
+    }
+  } else if (warp == 9) {
+    constexpr uint32_t id_s = idesc_f16(IsBf16<T>::v, 128, 128, 0, 0);
+    constexpr uint32_t id_o = idesc_f16(IsBf16<T>::v, 128, DP, 0, 1);
+    const uint32_t k_addr = smem_u32(sK), v_addr = smem_u32(sV);
+    int in = 0, qn = 0;
+    bool ok = true;
+    // waits for a tile of Q or g; rows behind the sequence's end are cleared, since their zero
+    // weights meet them in the accumulating products
+    auto arrived = [&](uint64_t* full, uint8_t* tiles, int i, int t, int site) -> bool {
+      const int s = i & 1;
+      if (!mbar_wait_warp(&full[s], (i >> 1) & 1, a.err, err_code(KERNEL_DKV, ROLE_MMA, site))) return false;
+      const int valid = (it.nq - t * a.tq) * a.group;
+      if (valid < a.group * a.tq) {
+        zero_rows_from<DP>(tiles + s * C::kTile, valid, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      tc_fence_after();
+      return true;
+    };
+    for (; ok && walk_item<true>(a, n, it); n += gridDim.x) {
+      const int tiles = it.kt1 - it.kt0;
+      if (tiles <= 0) continue;
+      ok = mbar_wait_warp(kv_full, in & 1, a.err, err_code(KERNEL_DKV, ROLE_MMA, 1));
+      ++in;
+      for (int j = -1; ok && j < tiles; ++j) {
+        // (j = -1: only the first tile's scores)
+        const int i = qn + j, s = i & 1;
+        if (j >= 0) {
+          ok = mbar_wait_warp(p_ready, i & 1, a.err, err_code(KERNEL_DKV, ROLE_MMA, 2));
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            mma_cols(tmem + 256, tmem, smem_u32(sG + s * C::kTile), id_o, j > 0);
+            umma_commit(&g_empty[s]);
+          }
+          __syncwarp();
+        }
+        if (j + 1 < tiles) {   // behind dV in the pipe, so S^T may overwrite P^T
+          ok = arrived(q_full, sQ, i + 1, it.kt0 + j + 1, 3);
+          if (!ok) break;
+          if (lane == 0) {
+            mma_rows(tmem, k_addr, smem_u32(sQ + ((i + 1) & 1) * C::kTile), id_s, a.ksteps);
+            umma_commit(s_full);
+          }
+          __syncwarp();
+        }
+        if (j >= 0) {
+          ok = mbar_wait_warp(ds_ready, i & 1, a.err, err_code(KERNEL_DKV, ROLE_MMA, 4));
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            mma_cols(tmem + 384, tmem + 128, smem_u32(sQ + s * C::kTile), id_o, j > 0);
+            umma_commit(&q_empty[s]);
+          }
+          __syncwarp();
+        }
+        if (j + 1 < tiles) {
+          ok = arrived(g_full, sG, i + 1, it.kt0 + j + 1, 5);
+          if (!ok) break;
+          if (lane == 0) {
+            mma_rows(tmem + 128, v_addr, smem_u32(sG + ((i + 1) & 1) * C::kTile), id_s, a.ksteps);
+            umma_commit(dp_full);
+          }
+          __syncwarp();
+        } else if (lane == 0) {
+          umma_commit(acc_full);
+          umma_commit(kv_empty);
+        }
+      }
+      qn += tiles;
+    }
+    if (lane == 0) {
+      umma_commit(drain);
+      mbar_wait_drain(drain, 0);
+    }
+  } else {
+    const int quad = warp & 3, half = warp >> 2;
+    const int row = quad * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const float c = a.scale * kLog2e;
+    T *dk = static_cast<T*>(a.dk), *dv = static_cast<T*>(a.dv);
+    if (a.walk == WALK_LIST) {
+      const long long per = static_cast<long long>(a.kv_heads) * a.dim / 8;
+      zero_outside(a.cu_k, a.seqs, a.kv_rows, per, dk, threadIdx.x, 256);
+      zero_outside(a.cu_k, a.seqs, a.kv_rows, per, dv, threadIdx.x, 256);
+    }
+    int qn = 0, in = 0;
+    bool ok = true;
+    for (; ok && walk_item<true>(a, n, it); n += gridDim.x) {
+      const int key = it.tile * kTileRows + row;
+      const bool live = key < it.klen;
+      const size_t orow = (static_cast<size_t>(it.k0) + key) * a.kv_heads + it.head;
+      bool on = live;
+      if (on && a.key_mask) on = a.key_mask[static_cast<size_t>(it.k0) + key] != 0;
+      const bool gone = __any_sync(0xffffffffu, !on);
+      for (int t = it.kt0; t < it.kt1; ++t, ++qn) {
+        const int cb = qn % C::kCols;
+        // queries in front of the first one that sees this key (causal): columns below `lo`
+        const int lo = a.causal ? max(0, min(kTileRows, (key - it.off - t * a.tq) * a.group)) : 0;
+        const bool cut = gone || __any_sync(0xffffffffu, lo > 0);
+        const float* col = sC + cb * 384;
+        ok = mbar_wait_warp(&c_full[cb], (qn / C::kCols) & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 1));
+        if (BIAS) ok = ok && mbar_wait_warp(b_full, qn & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 2));
+        ok = ok && mbar_wait_warp(s_full, qn & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 3));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t r[2][32];
+        FTM_TMEM_LD32_NOWAIT(lanes + half * 64, r[0]);
+        FTM_TMEM_LD32_NOWAIT(lanes + half * 64 + 32, r[1]);
+        tmem_wait_ld();
+        if (BIAS) {
+          // the bias of (query, this key): rows of the tile are queries
+          const uint8_t* bt = sB + (row >> 6) * kBlk + (row & 7) * 2;
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const int cq = half * 64 + q * 32 + e;
+              const T bv = *reinterpret_cast<const T*>(bt + sw128_off(cq, (row & 63) >> 3));
+              r[q][e] = __float_as_uint(fmaf(__uint_as_float(r[q][e]), a.scale, static_cast<float>(bv)));
+            }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(b_empty);
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const int cq = half * 64 + q * 32 + e;
+            const float4 x4 = *reinterpret_cast<const float4*>(col + cq);
+            const float xs[4] = {x4.x, x4.y, x4.z, x4.w};
+            float ys[4] = {0.f, 0.f, 0.f, 0.f};
+            if (BIAS) {
+              const float4 y4 = *reinterpret_cast<const float4*>(col + 128 + cq);
+              ys[0] = y4.x; ys[1] = y4.y; ys[2] = y4.z; ys[3] = y4.w;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float x = __uint_as_float(r[q][e + k]);
+              r[q][e + k] = __float_as_uint(ex2(BIAS ? fmaf(x - xs[k], kLog2e, -ys[k]) : fmaf(x, c, -xs[k])));
+            }
+          }
+        if (cut) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const uint32_t bits = on ? ~bits_below(lo, half * 2 + q) : 0u;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((bits >> e) & 1u)) r[q][e] = 0u;
+          }
+        }
+        uint32_t pk[32];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            pk[q * 16 + e / 2] = pack16<T>(__uint_as_float(r[q][e]), __uint_as_float(r[q][e + 1]));
+        named_barrier_sync(1 + quad, 64);   // both halves have read S^T: P^T goes over it
+        tmem_st32(lanes + half * 32, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready);
+        ok = mbar_wait_warp(dp_full, qn & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 4));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t d[32];
+          FTM_TMEM_LD32_NOWAIT(lanes + 128 + half * 64 + q * 32, d);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 z = *reinterpret_cast<const float4*>(col + 256 + half * 64 + q * 32 + e);
+            const float zs[4] = {z.x, z.y, z.z, z.w};
+            float x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              x[k] = __uint_as_float(r[q][e + k]) * (__uint_as_float(d[e + k]) - zs[k]);
+              if (cut) x[k] = r[q][e + k] ? x[k] : 0.f;
+            }
+            pk[q * 16 + e / 2] = pack16<T>(x[0], x[1]);
+            pk[q * 16 + e / 2 + 1] = pack16<T>(x[2], x[3]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c_empty[cb]);
+        named_barrier_sync(1 + quad, 64);
+        tmem_st32(lanes + 128 + half * 32, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready);
+      }
+      if (!ok) break;
+      const bool any = it.kt1 > it.kt0;
+      if (any) {
+        ok = mbar_wait_warp(acc_full, in & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 5));
+        if (!ok) break;
+        ++in;
+        tc_fence_after();
+      }
+      store_acc<DP / 2>(lanes + 256, half * (DP / 2), a.dim, 1.f, live, any, dv + orow * a.dim);
+      store_acc<DP / 2>(lanes + 384, half * (DP / 2), a.dim, a.scale, live, any, dk + orow * a.dim);
+      tc_fence_before();
+    }
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------------------ dbias
+template <int DP>
+struct DbCfg {
+  static constexpr int kTile = DP / 64 * kBlk;
+  static constexpr int kStages = DP == 64 ? 2 : 1;
+  static constexpr int kStage = 4 * kTile;    // Q, g, K, V
+  static constexpr int kOffB = kStages * kStage;
+  static constexpr int kOffBar = kOffB + 2 * kBlk;
+  static constexpr int kSmem = kOffBar + 256 + 1024;
+};
+
+template <int DP, typename T>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnArgs a) {
+  using C = DbCfg<DP>;
+  constexpr int NS = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sB = smem + C::kOffB;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* empty = full + 2;
+  uint64_t* t_full = full + 4;
+  uint64_t* t_empty = full + 6;
+  uint64_t* b_full = full + 8;
+  uint64_t* b_empty = full + 9;
+  uint64_t* drain = full + 10;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + 11);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 11; ++i) mbar_init(full + i, i == 6 || i == 7 || i == 9 ? 8 : 1);
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dep_wait();
+  grid_dep_release();
+
+  const int biases = a.seqs / a.bias_seqs;
+  const int items = a.splits * biases * a.heads * a.q_tiles * a.k_tiles;
+  int split = 0, bb = 0, head = 0, qt = 0, kt = 0, r0 = 0, r1 = 0;
+  auto item = [&](int i) {
+    kt = i % a.k_tiles;
+    i /= a.k_tiles;
+    qt = i % a.q_tiles;
+    i /= a.q_tiles;
+    head = i % a.heads;
+    i /= a.heads;
+    bb = i % biases;
+    split = i / biases;
+    r0 = static_cast<int>(static_cast<long long>(a.bias_seqs) * split / a.splits);
+    r1 = static_cast<int>(static_cast<long long>(a.bias_seqs) * (split + 1) / a.splits);
+  };
+
+  if (warp == 8) {
+    if (lane == 0) {
+      int rn = 0, in = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+        item(i);
+        ok = mbar_wait(b_empty, (in & 1) ^ 1, a.err, err_code(KERNEL_DBIAS, ROLE_PRODUCER, 1));
+        if (!ok) break;
+        mbar_arrive_expect_tx(b_full, 2 * kBlk);
+        for (int h = 0; h < 2; ++h)
+          tma_load_4d(&maps.bias, b_full, sB + h * kBlk, kt * kTileRows + h * 64, qt * kTileRows, head, bb);
+        ++in;
+        for (int r = r0; r < r1; ++r, ++rn) {
+          const int s = rn % NS;
+          ok = mbar_wait(&empty[s], ((rn / NS) & 1) ^ 1, a.err, err_code(KERNEL_DBIAS, ROLE_PRODUCER, 2));
+          if (!ok) break;
+          const int seq = bb * a.bias_seqs + r;
+          const int q0 = seq * a.q_len + qt * kTileRows, k0 = seq * a.k_len + kt * kTileRows;
+          uint8_t* st = smem + s * C::kStage;
+          mbar_arrive_expect_tx(&full[s], C::kStage);
+          load_tile4<DP>(&maps.q, &full[s], st, 0, head, q0);
+          load_tile4<DP>(&maps.g, &full[s], st + C::kTile, 0, head, q0);
+          load_tile4<DP>(&maps.k, &full[s], st + 2 * C::kTile, head, k0, 0);
+          load_tile4<DP>(&maps.v, &full[s], st + 3 * C::kTile, head, k0, 0);
+        }
+      }
+      for (int i = rn > NS ? rn - NS : 0; i < rn; ++i) mbar_wait_drain(&full[i % NS], (i / NS) & 1);
+      if (in) mbar_wait_drain(b_full, (in - 1) & 1);
+    }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      constexpr uint32_t id_s = idesc_f16(IsBf16<T>::v, 128, 128, 0, 0);
+      int rn = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+        item(i);
+        for (int r = r0; r < r1; ++r, ++rn) {
+          const int s = rn % NS, tb = rn & 1;
+          ok = mbar_wait(&full[s], (rn / NS) & 1, a.err, err_code(KERNEL_DBIAS, ROLE_MMA, 1)) &&
+               mbar_wait(&t_empty[tb], ((rn >> 1) & 1) ^ 1, a.err, err_code(KERNEL_DBIAS, ROLE_MMA, 2));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + s * C::kStage);
+          mma_rows(tmem + tb * 256, st, st + 2 * C::kTile, id_s, a.ksteps);
+          mma_rows(tmem + tb * 256 + 128, st + C::kTile, st + 3 * C::kTile, id_s, a.ksteps);
+          umma_commit(&t_full[tb]);
+          umma_commit(&empty[s]);
+        }
+      }
+      umma_commit(drain);
+      mbar_wait_drain(drain, 0);
+    }
+  } else {
+    const int quad = warp & 3, half = warp >> 2;
+    const int row = quad * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    int rn = 0, in = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+      item(i);
+      const int pos = qt * kTileRows + row;
+      const bool live = pos < a.q_len;
+      Item it;
+      it.klen = a.k_len;
+      ok = mbar_wait_warp(b_full, in & 1, a.err, err_code(KERNEL_DBIAS, ROLE_EPILOGUE, 1));
+      if (!ok) break;
+      ++in;
+      float acc[64];
+#pragma unroll
+      for (int e = 0; e < 64; ++e) acc[e] = 0.f;
+      for (int r = r0; r < r1; ++r, ++rn) {
+        const int tb = rn & 1, seq = bb * a.bias_seqs + r;
+        it.k0 = seq * a.k_len;
+        uint32_t keep[4];
+        key_bits(a, it, kt, lane, keep);
+        const float4 st = live ? a.bstats[(static_cast<size_t>(seq) * a.q_len + pos) * a.heads + head]
+                               : make_float4(0.f, INFINITY, 0.f, 0.f);
+        ok = mbar_wait_warp(&t_full[tb], (rn >> 1) & 1, a.err, err_code(KERNEL_DBIAS, ROLE_EPILOGUE, 2));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t x[32], d[32];
+          FTM_TMEM_LD32_NOWAIT(lanes + tb * 256 + half * 64 + q * 32, x);
+          FTM_TMEM_LD32_NOWAIT(lanes + tb * 256 + 128 + half * 64 + q * 32, d);
+          tmem_wait_ld();
+          const uint32_t on = keep[half * 2 + q];
+#pragma unroll
+          for (int e8 = 0; e8 < 4; ++e8) {
+            float f[8];
+            unpack8(*reinterpret_cast<const uint4*>(sB + half * kBlk + sw128_off(row, q * 4 + e8)), IsBf16<T>::v, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int k = e8 * 8 + e;
+              const float t = fmaf(__uint_as_float(x[k]), a.scale, f[e]);
+              const float p = ex2(fmaf(t - st.x, kLog2e, -st.y));
+              const float ds = p * (__uint_as_float(d[k]) - st.z);
+              acc[q * 32 + k] += (on >> k) & 1u ? ds : 0.f;
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&t_empty[tb]);
+      }
+      if (!ok) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b_empty);
+      if (live) {
+        const size_t at = ((static_cast<size_t>(bb) * a.heads + head) * a.q_len + pos) * a.k_len;
+        const size_t all = static_cast<size_t>(biases) * a.heads * a.q_len * a.k_len;
+#pragma unroll
+        for (int e = 0; e < 64; ++e) {
+          const int col = kt * kTileRows + half * 64 + e;
+          if (col >= a.k_len) break;
+          if (a.splits == 1) static_cast<T*>(a.dbias)[at + col] = T(acc[e]);
+          else a.dbias_part[split * all + at + col] = acc[e];
+        }
+      }
+    }
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// dbias = sum of the splits' parts, in order
+template <typename T>
+__global__ void __launch_bounds__(256)
+attn_dbias_reduce_kernel(const float* __restrict__ part, T* __restrict__ out, long long n, int splits) {
+  grid_dep_wait();
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * 256) {
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k) s += part[k * n + i];
+    out[i] = T(s);
+  }
+  grid_dep_release();
+}
+
+int item_grid(const AttnLaunch& l, bool kv) {
+  const AttnArgs& a = l.a;
+  long long items;
+  if (a.walk == WALK_LIST)
+    items = ((kv ? (static_cast<long long>(a.kv_rows) + kTileRows - 1) / kTileRows
+                 : (static_cast<long long>(a.q_rows) + a.tq - 1) / a.tq) + a.seqs) * a.kv_heads;
+  else
+    items = static_cast<long long>(a.seqs) * (kv ? a.k_tiles : a.q_tiles) * a.kv_heads;
+  return static_cast<int>(items < l.sms ? items : l.sms);
+}
+
+template <typename Kern>
+cudaError_t go(Kern kern, const AttnLaunch& l, int grid, int smem) {
+  const cudaError_t e = set_smem_once(reinterpret_cast<const void*>(kern), smem);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kern, dim3(grid), dim3(kBwdThreads), smem, l.stream, nullptr, 0, l.m, l.a);
+}
+
+}  // namespace
+
+cudaError_t launch_attn_delta(const AttnLaunch& l) {
+  const int lanes = l.a.dim <= 32 ? 4 : l.a.dim <= 64 ? 8 : 16;
+  const long long per = 256 / lanes, n = static_cast<long long>(l.a.q_rows) * l.a.heads;
+  const long long need = (n + per - 1) / per, cap = static_cast<long long>(l.sms) * 8;
+  const dim3 grid(static_cast<unsigned>(need < cap ? need : cap));
+  if (l.bf16) return launch_pdl(attn_delta_kernel<__nv_bfloat16>, grid, dim3(256), 0, l.stream, nullptr, 0, l.a, lanes, l.bias);
+  return launch_pdl(attn_delta_kernel<__half>, grid, dim3(256), 0, l.stream, nullptr, 0, l.a, lanes, l.bias);
+}
+
+#define FTM_BY_SHAPE(KERN, CFG, GRID)                                                                        \
+  if (l.dp == 64) {                                                                                          \
+    if (l.bias) return l.bf16 ? go(KERN<64, true, __nv_bfloat16>, l, GRID, CFG(64, true)) : go(KERN<64, true, __half>, l, GRID, CFG(64, true));       \
+    return l.bf16 ? go(KERN<64, false, __nv_bfloat16>, l, GRID, CFG(64, false)) : go(KERN<64, false, __half>, l, GRID, CFG(64, false));               \
+  }                                                                                                          \
+  if (l.bias) return l.bf16 ? go(KERN<128, true, __nv_bfloat16>, l, GRID, CFG(128, true)) : go(KERN<128, true, __half>, l, GRID, CFG(128, true));     \
+  return l.bf16 ? go(KERN<128, false, __nv_bfloat16>, l, GRID, CFG(128, false)) : go(KERN<128, false, __half>, l, GRID, CFG(128, false));
+
+cudaError_t launch_attn_dq(const AttnLaunch& l) {
+  const int grid = item_grid(l, false);
+#define DQ_SMEM(D, B) (DqCfg<D, B>::kSmem)
+  FTM_BY_SHAPE(attn_dq_kernel, DQ_SMEM, grid)
+}
+
+cudaError_t launch_attn_dkv(const AttnLaunch& l) {
+  const int grid = item_grid(l, true);
+#define DKV_SMEM(D, B) (DkvCfg<D, B>::kSmem)
+  FTM_BY_SHAPE(attn_dkv_kernel, DKV_SMEM, grid)
+}
+
+cudaError_t launch_attn_dbias(const AttnLaunch& l) {
+  const AttnArgs& a = l.a;
+  const int biases = a.seqs / a.bias_seqs;
+  const long long items = static_cast<long long>(a.splits) * biases * a.heads * a.q_tiles * a.k_tiles;
+  const int grid = static_cast<int>(items < l.sms ? items : l.sms);
+  cudaError_t e;
+  if (l.dp == 64)
+    e = l.bf16 ? go(attn_dbias_kernel<64, __nv_bfloat16>, l, grid, DbCfg<64>::kSmem)
+               : go(attn_dbias_kernel<64, __half>, l, grid, DbCfg<64>::kSmem);
+  else
+    e = l.bf16 ? go(attn_dbias_kernel<128, __nv_bfloat16>, l, grid, DbCfg<128>::kSmem)
+               : go(attn_dbias_kernel<128, __half>, l, grid, DbCfg<128>::kSmem);
+  if (e != cudaSuccess || a.splits == 1) return e;
+  const long long n = static_cast<long long>(biases) * a.heads * a.q_len * a.k_len;
+  const long long need = (n + 255) / 256, cap = static_cast<long long>(l.sms) * 8;
+  const dim3 rg(static_cast<unsigned>(need < cap ? need : cap));
+  if (l.bf16)
+    return launch_pdl(attn_dbias_reduce_kernel<__nv_bfloat16>, rg, dim3(256), 0, l.stream, nullptr, 0,
+                      static_cast<const float*>(a.dbias_part), static_cast<__nv_bfloat16*>(a.dbias), n, a.splits);
+  return launch_pdl(attn_dbias_reduce_kernel<__half>, rg, dim3(256), 0, l.stream, nullptr, 0,
+                    static_cast<const float*>(a.dbias_part), static_cast<__half*>(a.dbias), n, a.splits);
+}
+
+}  // namespace ftm

@@ -130,6 +130,11 @@ cudaError_t launch_output_stage(const CUtensorMap& zmap, const CUtensorMap& xmap
 // entry): problem, rows == cols, non-null 16-byte-aligned z / packed / out / mask.
 int check_forward_args(const ftm_problem* p, const void* z, const float* mask, const void* packed,
                        const void* out);
+// Tiled tensor map (128-byte swizzle) of 16-bit elements over `rank` <= 5 dimensions, strides
+// in bytes for dimensions 1 and up; false when the driver refuses it.
+bool make_tensor_map(CUtensorMap* m, bool bf16, int rank, const void* base, const uint64_t* dims,
+                     const uint64_t* strides, const uint32_t* box);
+int device_sms(int dev);
 // What ftm_last_launch_count() reports for the calling thread.
 void set_last_launch_count(int n);
 

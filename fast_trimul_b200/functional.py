@@ -13,11 +13,15 @@ runs the torch formula with the reference's casts.
 
 Beside it, the other operators of a pair / single representation trunk:
 
-    layer_norm(x, weight, bias, eps)        (ops/norm.py)
+    layer_norm(x, weight, bias, eps)                                  (ops/norm.py)
+    pair_attention(q, k, v, bias, mask)                               (ops/attention.py)
+    packed_attention(q, k, v, cu_seqlens, cu_seqlens_k, causal=...)
+    cached_attention(q, k_cache, v_cache, lengths)
 """
 
 import torch
 
+from .ops.attention import cached_attention, packed_attention, pair_attention  # noqa: F401
 from .ops.norm import layer_norm  # noqa: F401
 
 

@@ -1,0 +1,375 @@
+"""Attention on the sm_100a kernels: packed sequences, one new token over a cache, and rows
+of a pair representation with a shared bias.
+
+* `packed_attention` -- sequences of different lengths stored one behind the other, grouped
+  key / value heads, causal or not; forward and backward.
+* `cached_attention` -- its form for single tokens: one query per sequence over a key / value
+  cache whose lengths live on the device; no backward.
+* `pair_attention`   -- attention of every row of a pair representation, with an additive bias
+  that all rows of a batch element share and a mask of the keys (triangle attention, and
+  with one row the single representation's attention with pair bias); forward and backward,
+  the bias' gradient included.
+
+On CUDA tensors the kernels take fp16 and bf16 with a head dimension that is a multiple of 8
+up to 128, and raise `NativeDeclined` for anything else; sums, softmax statistics and
+gradients' accumulators are fp32. Elsewhere the formula runs in torch, in fp32. A query that
+sees no key gives zeros, and masked keys count as absent whatever K and V hold there.
+"""
+
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from .norm import device_guard
+
+_DT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+class HostErrorWord:
+    """The error word of the attention kernels of one GPU, in pinned host memory that the
+    kernels write directly: the next call (or `check`) sees an expired wait with a plain read,
+    and no call has to copy anything."""
+
+    def __init__(self):
+        self.host = torch.zeros(16, dtype=torch.int32).pin_memory()
+        self.ptr = self.host.data_ptr()
+        self.word = ctypes.c_int32.from_address(self.ptr)
+
+    def poll(self):
+        code = self.word.value
+        if code:
+            self.word.value = 0
+            raise _lib.NativeKernelError(
+                f"a bounded device wait expired in a native attention kernel (code 0x{code:x}: kernel "
+                f"{code >> 8}, role {(code >> 4) & 15}, site {code & 15}); its output is invalid")
+
+    def check(self):
+        torch.cuda.synchronize()
+        self.poll()
+
+
+_ERROR_WORDS = {}
+
+
+def attention_error_word(device=None):
+    """The HostErrorWord of a GPU (default: the current one)."""
+    index = torch.cuda.current_device() if device is None or device.index is None else device.index
+    w = _ERROR_WORDS.get(index)
+    if w is None:
+        w = _ERROR_WORDS[index] = HostErrorWord()
+    return w
+
+
+# --------------------------------------------------------------------------- checks
+def _scale(scale, dim):
+    s = dim ** -0.5 if scale is None else float(scale)
+    if not (math.isfinite(s) and s >= 0):
+        raise ValueError(f"scale must be finite and not negative, got {scale}")
+    return s
+
+
+def _same(device, dtype, **tensors):
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, q on {device}")
+        if dtype is not None and t.dtype != dtype:
+            raise ValueError(f"{name} is {t.dtype}, q {dtype}")
+
+
+def _heads(q_heads, kv_heads, dim, cuda, dtype):
+    if kv_heads < 1 or q_heads < 1 or q_heads % kv_heads:
+        raise ValueError(f"{q_heads} query heads cannot share {kv_heads} key / value heads")
+    if dim < 1:
+        raise ValueError("the head dimension is empty")
+    if not cuda:
+        return
+    if dtype not in _DT:
+        raise _lib.NativeDeclined(f"attention kernels take fp16 and bf16, got {dtype}")
+    if dim % 8 or dim > 128:
+        raise _lib.NativeDeclined(f"attention kernels take head dimensions that are multiples of 8 up to 128, got {dim}")
+    if q_heads // kv_heads > 128:
+        raise _lib.NativeDeclined("at most 128 query heads per key / value head")
+
+
+def _in_place(t):
+    """`t` if the kernels can read it where it is (dense, 16-byte aligned vectors of the last
+    dimension, any other strides of whole vectors), else a contiguous copy."""
+    st, sh = t.stride(), t.shape
+    if st[-1] != 1 or t.data_ptr() % 16:
+        return t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 == 0 else t.clone()
+    for s, n in zip(st[:-1], sh[:-1]):
+        if n > 1 and (s <= 0 or s % 8):
+            return t.contiguous()
+    return t
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class _Call:
+    """What a forward and its backward share beside the tensors: the C problem's plain fields
+    and the device arrays it points to."""
+
+    __slots__ = ("heads", "kv_heads", "dim", "causal", "scale", "seqs", "q_len", "kv_len", "cu_q", "cu_k",
+                 "lengths", "mask", "bias_seqs")
+
+    def problem(self, q, k, v, bias, out, stats):
+        """q (rows, heads, dim); k, v (rows, heads, dim) or (batch, rows, heads, dim)."""
+        b = k.dim() == 4
+        br, bh, bb = (bias.stride(2), bias.stride(1), bias.stride(0)) if bias is not None else (0, 0, 0)
+        return _lib.Attention(
+            _DT[q.dtype], self.heads, self.kv_heads, self.dim, self.causal, self.scale, self.seqs, self.q_len,
+            self.kv_len, q.shape[0], k.shape[-3], _ptr(self.cu_q), _ptr(self.cu_k), _ptr(self.lengths),
+            q.data_ptr(), q.stride(0), q.stride(1),
+            k.data_ptr(), k.stride(-3), k.stride(-2), k.stride(0) if b else 0,
+            v.data_ptr(), v.stride(-3), v.stride(-2), v.stride(0) if b else 0,
+            _ptr(self.mask), _ptr(bias), self.bias_seqs, br, bh, bb, out.data_ptr(), _ptr(stats))
+
+
+def _launch(call, q, k, v, bias, train):
+    """Forward launch; returns out, the row statistics and the packed call's tile lists (the
+    last two only when training)."""
+    lib = _lib.load()
+    dev = q.device
+    err = attention_error_word(dev)
+    err.poll()
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    stats = torch.empty(q.shape[0], call.heads, 2, dtype=torch.float32, device=dev) if train else None
+    with device_guard(q):
+        prob = call.problem(q, k, v, bias, out, stats)
+        nbytes = lib.ftm_attention_workspace_bytes(prob, train)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _lib.check(lib.ftm_attention_fwd(prob, train, _ptr(ws), nbytes, err.ptr,
+                                         torch.cuda.current_stream().cuda_stream), "ftm_attention_fwd")
+    _lib.record_launches()
+    return out, stats, ws
+
+
+class _Attention(torch.autograd.Function):
+    """Forward that keeps its output and two floats of statistics per row and head; the backward
+    recomputes the weights tile by tile. No atomics: the gradients are the same bits on every
+    call, and those of shared heads and of a shared bias are summed inside the kernels."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, bias, call):
+        q, k, v = _in_place(q), _in_place(k), _in_place(v)
+        ready = None if bias is None else _bias_in_place(bias)
+        out, stats, lists = _launch(call, q, k, v, ready, 1)
+        ctx.call = call
+        ctx.bias_shape = None if bias is None else bias.shape
+        ctx.save_for_backward(q, k, v, ready, out, stats, lists)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, k, v, bias, out, stats, lists = ctx.saved_tensors
+        lib = _lib.load()
+        call, dev = ctx.call, q.device
+        err = attention_error_word(dev)
+        err.poll()
+        need_q, need_k, need_v, need_b = ctx.needs_input_grad[:4]
+        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)   # noqa: E731
+        grad = _in_place(grad if grad.dtype == q.dtype else grad.to(q.dtype))
+        dq = new(q) if need_q else None
+        dk, dv = (new(k), new(v)) if need_k or need_v else (None, None)
+        db = torch.empty(ctx.bias_shape, dtype=q.dtype, device=dev) if need_b else None
+        with device_guard(q):
+            prob = call.problem(q, k, v, bias, out, stats)
+            nbytes = lib.ftm_attention_bwd_workspace_bytes(prob, 1 if need_b else 0)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            _lib.check(lib.ftm_attention_bwd(
+                prob, grad.data_ptr(), grad.stride(0), grad.stride(1), _ptr(lists),
+                0 if lists is None else lists.numel(), ws.data_ptr(), nbytes, _ptr(dq), _ptr(dk), _ptr(dv),
+                _ptr(db), err.ptr, torch.cuda.current_stream().cuda_stream), "ftm_attention_bwd")
+        _lib.record_launches()
+        return dq, dk if need_k else None, dv if need_v else None, db, None
+
+
+def _run(call, q, k, v, bias):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    (bias is not None and bias.requires_grad)):
+        return _Attention.apply(q, k, v, bias, call)
+    return _launch(call, _in_place(q), _in_place(k), _in_place(v),
+                   None if bias is None else _bias_in_place(bias), 0)[0]
+
+
+def _as_mask(mask, device, shape, name):
+    if mask.device != device:
+        raise ValueError(f"{name} is on {mask.device}, q on {device}")
+    if tuple(mask.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(mask.shape)}")
+    return mask if mask.dtype == torch.bool else mask != 0
+
+
+def _attend(q, k, v, keep, scale, bias=None):
+    """The formula in torch: q, k, v (..., length, dim) fp32, keep broadcastable to the scores."""
+    s = (q @ k.transpose(-1, -2)) * scale
+    if bias is not None:
+        s = s + bias
+    s = torch.where(keep, s, torch.full_like(s, -math.inf))
+    top = s.detach().amax(-1, keepdim=True)
+    top = torch.where(top == -math.inf, torch.zeros_like(top), top)
+    p = torch.exp(s - top)
+    total = p.sum(-1, keepdim=True)
+    return (p / torch.where(total == 0, torch.ones_like(total), total)) @ v
+
+
+# --------------------------------------------------------------------------- packed
+def _ends(cu, device, name):
+    if cu.dim() != 1 or cu.numel() < 1 or cu.dtype.is_floating_point or cu.dtype == torch.bool:
+        raise ValueError(f"{name} must be a vector of whole numbers, got {cu.dtype} {tuple(cu.shape)}")
+    if cu.device != device:
+        raise ValueError(f"{name} is on {cu.device}, q on {device}")
+    return cu.to(torch.int32).contiguous()
+
+
+def _packed_torch(q, k, v, cu_q, cu_k, causal, scale, mask):
+    out = torch.zeros(q.shape, dtype=torch.float32, device=q.device)
+    group = q.shape[1] // k.shape[1]
+    pieces, at = [], 0
+    for i in range(cu_q.numel() - 1):
+        a, c = int(cu_q[i]), int(cu_k[i])
+        b, d = int(cu_q[i + 1]), int(cu_k[i + 1])
+        qs, n, m = q[a:b].float().transpose(0, 1), b - a, d - c
+        keep = torch.ones(n, m, dtype=torch.bool, device=q.device)
+        if causal:
+            keep = keep.tril(m - n)
+        if mask is not None:
+            keep = keep & mask[c:d]
+        rows = lambda t: (t[c:d].float() if mask is None else   # noqa: E731
+                          t[c:d].float().masked_fill(~mask[c:d, None, None], 0)
+                          ).transpose(0, 1).repeat_interleave(group, 0)
+        if m == 0:
+            o = qs * 0
+        else:
+            o = _attend(qs, rows(k), rows(v), keep, scale)
+        pieces += [out[at:a], o.transpose(0, 1)]
+        at = b
+    return torch.cat([*pieces, out[at:]]).to(q.dtype)
+
+
+def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, *, causal=True, scale=None, key_mask=None):
+    """Attention within each of B packed sequences.
+
+    q: (rows, heads, dim); k, v: (rows, kv_heads, dim) with heads a multiple of kv_heads (query
+    head h reads head h // (heads / kv_heads)). Sequence i is rows cu_seqlens[i] to
+    cu_seqlens[i + 1] of q and the same rows of k and v, or cu_seqlens_k's: whole numbers on q's
+    device that do not descend. Rows of no sequence give zeros. `causal`: query i of a sequence
+    sees keys j <= i + (keys - queries), aligned to the last key, so a prompt's continuation
+    passes its new queries and all keys. scale: dim ** -0.5 if None. key_mask: (rows of k,), keys
+    with 0 / False are not seen. Returns q's shape and type. Differentiable once in q, k and v."""
+    if q.dim() != 3 or k.dim() != 3 or tuple(k.shape) != tuple(v.shape) or q.shape[2] != k.shape[2]:
+        raise ValueError("packed_attention needs q (rows, heads, dim) and k, v (rows, kv_heads, dim), got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    _heads(q.shape[1], k.shape[1], q.shape[2], q.is_cuda, q.dtype)
+    _same(q.device, q.dtype, k=k, v=v)
+    s = _scale(scale, q.shape[2])
+    cu_q = _ends(cu_seqlens, q.device, "cu_seqlens")
+    if cu_seqlens_k is None and q.shape[0] != k.shape[0]:
+        raise ValueError("q and k have different numbers of rows: cu_seqlens_k is needed")
+    cu_k = cu_q if cu_seqlens_k is None else _ends(cu_seqlens_k, q.device, "cu_seqlens_k")
+    if cu_q.numel() != cu_k.numel():
+        raise ValueError(f"{cu_q.numel() - 1} query sequences, {cu_k.numel() - 1} key sequences")
+    mask = None if key_mask is None else _as_mask(key_mask, q.device, (k.shape[0],), "key_mask")
+    if not q.is_cuda:
+        return _packed_torch(q, k, v, cu_q, cu_k, causal, s, mask)
+    if cu_q.numel() < 2 or q.shape[0] == 0 or k.shape[0] == 0:
+        return q * 0 + (k.sum() + v.sum()) * 0 if torch.is_grad_enabled() else torch.zeros_like(q)
+    c = _Call()
+    c.heads, c.kv_heads, c.dim, c.causal, c.scale = q.shape[1], k.shape[1], q.shape[2], bool(causal), s
+    c.seqs, c.q_len, c.kv_len, c.cu_q, c.cu_k, c.lengths = cu_q.numel() - 1, 0, 0, cu_q, cu_k, None
+    c.mask, c.bias_seqs = None if mask is None else mask.contiguous(), 0
+    return _run(c, q, k, v, None)
+
+
+# --------------------------------------------------------------------------- cached
+def cached_attention(q, k_cache, v_cache, lengths, *, scale=None):
+    """One new token of each sequence over its cache.
+
+    q: (B, heads, dim); k_cache, v_cache: (B, capacity, kv_heads, dim), the new token's key and
+    value included; lengths: (B,) whole numbers on q's device, how many positions of each cache
+    hold keys (read on the device, clamped to 0 .. capacity: a captured graph replays with new
+    lengths). A sequence of length 0 gives zeros. Returns (B, heads, dim). For inference: there is
+    no backward, and inputs that want gradients are refused."""
+    if q.dim() != 3 or k_cache.dim() != 4 or tuple(k_cache.shape) != tuple(v_cache.shape) or \
+            q.shape[0] != k_cache.shape[0] or q.shape[2] != k_cache.shape[3]:
+        raise ValueError("cached_attention needs q (B, heads, dim) and caches (B, capacity, kv_heads, dim), got "
+                         f"{tuple(q.shape)}, {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    B, H, D = q.shape
+    L, HK = k_cache.shape[1], k_cache.shape[2]
+    _heads(H, HK, D, q.is_cuda, q.dtype)
+    _same(q.device, q.dtype, k_cache=k_cache, v_cache=v_cache)
+    s = _scale(scale, D)
+    lens = _ends(lengths, q.device, "lengths") if B else lengths
+    if tuple(lens.shape) != (B,):
+        raise ValueError(f"lengths must have shape ({B},), got {tuple(lens.shape)}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_cache, v_cache)):
+        raise ValueError("cached_attention has no backward: call it under torch.no_grad()")
+    if B == 0 or L == 0:
+        return torch.zeros_like(q)
+    if not q.is_cuda:
+        keep = torch.arange(L, device=q.device) < lens[:, None]
+        rows = lambda t: t.float().masked_fill(~keep[..., None, None], 0).transpose(1, 2)   # noqa: E731
+        o = _attend(q.float().view(B, HK, H // HK, D), rows(k_cache), rows(v_cache), keep[:, None, None], s)
+        return o.reshape(B, H, D).to(q.dtype)
+    c = _Call()
+    c.heads, c.kv_heads, c.dim, c.causal, c.scale = H, HK, D, False, s
+    c.seqs, c.q_len, c.kv_len, c.cu_q, c.cu_k, c.lengths = B, 1, 0, None, None, lens
+    c.mask, c.bias_seqs = None, 0
+    return _launch(c, _in_place(q), _in_place(k_cache), _in_place(v_cache), None, 0)[0]
+
+
+# ----------------------------------------------------------------------------- pair
+def _bias_in_place(bias):
+    """(B, heads, N, N) with rows a multiple of 8 elements apart: copied when they are not."""
+    n = bias.shape[-1]
+    if n % 8 == 0:
+        return _in_place(bias)
+    if bias.stride(-1) == 1 and bias.data_ptr() % 16 == 0 and \
+            all(s > 0 and s % 8 == 0 for s, e in zip(bias.stride()[:-1], bias.shape[:-1]) if e > 1):
+        return bias
+    wide = torch.empty(*bias.shape[:-1], (n + 7) // 8 * 8, dtype=bias.dtype, device=bias.device)
+    wide[..., :n] = bias
+    return wide[..., :n]
+
+
+def pair_attention(q, k, v, bias, mask=None, *, scale=None):
+    """Attention along the rows of a pair representation, with a bias that the rows share.
+
+    q, k, v: (B, R, N, heads, dim) -- each of the B * R rows attends within itself; bias: (B or 1,
+    heads, N, N), added to the scaled scores of every row, or None; mask: (B, R, N), keys with 0 /
+    False are not seen (a row that has none left gives zeros). scale: dim ** -0.5 if None. Returns
+    q's shape and type. Triangle attention has R = N; R = 1 is attention of a single representation
+    with pair bias. Differentiable once in q, k, v and bias (its gradient summed over the rows)."""
+    if q.dim() != 5 or tuple(k.shape) != tuple(q.shape) or tuple(v.shape) != tuple(q.shape):
+        raise ValueError("pair_attention needs q, k and v of one shape (B, R, N, heads, dim), got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, R, N, H, D = q.shape
+    _heads(H, H, D, q.is_cuda, q.dtype)
+    _same(q.device, q.dtype, k=k, v=v, bias=bias)
+    s = _scale(scale, D)
+    if bias is not None and (bias.dim() != 4 or bias.shape[0] not in (1, B) or tuple(bias.shape[1:]) != (H, N, N)):
+        raise ValueError(f"bias must have shape ({B} or 1, {H}, {N}, {N}), got {tuple(bias.shape)}")
+    m = None if mask is None else _as_mask(mask, q.device, (B, R, N), "mask")
+    if q.numel() == 0:
+        return q * 0 if bias is None else q * 0 + bias.sum() * 0
+    if not q.is_cuda:
+        keep = torch.ones(B, R, N, dtype=torch.bool, device=q.device) if m is None else m
+        rows = lambda t: t.float().masked_fill(~keep[..., None, None], 0).transpose(2, 3)   # noqa: E731
+        o = _attend(q.float().transpose(2, 3), rows(k), rows(v), keep[:, :, None, None, :], s,
+                    None if bias is None else bias.float()[:, None])
+        return o.transpose(2, 3).to(q.dtype)
+    c = _Call()
+    c.heads, c.kv_heads, c.dim, c.causal, c.scale = H, H, D, False, s
+    c.seqs, c.q_len, c.kv_len, c.cu_q, c.cu_k, c.lengths = B * R, N, N, None, None, None
+    c.mask = None if m is None else m.contiguous()
+    c.bias_seqs = 0 if bias is None else B * R // bias.shape[0]
+    flat = lambda t: t.reshape(B * R * N, H, D)   # noqa: E731
+    return _run(c, flat(q), flat(k), flat(v), bias).view(B, R, N, H, D)

@@ -350,6 +350,59 @@ int ftm_layer_norm_bwd(const void* x, int32_t dtype, int64_t x_row_stride, const
                        void* workspace, size_t workspace_bytes, int64_t rows, int32_t width,
                        ftm_stream_t stream);
 
+/* ---- attention ----------------------------------------------------------------
+ * No counterpart in the reference. o = softmax(scale q k^T + bias) v for `sequences`
+ * independent sequences of fp16 or bf16 rows; query head h reads key / value head
+ * h / (heads / kv_heads). A query without any visible key gives zeros. Which rows make a
+ * sequence:
+ *   packed   cu_q, cu_k (device, sequences + 1 each): rows [cu[i], cu[i+1]); rows in front of
+ *            cu[0] and behind cu[sequences] belong to none (their outputs and gradients are 0).
+ *            Values are clamped to the tensors on the device, whatever they are.
+ *   uniform  cu_q = cu_k = NULL: q_len / kv_len consecutive rows each.
+ *   cache    kv_lengths (device, one per sequence): one query row per sequence (q_len 1), keys
+ *            [0, kv_lengths[i]) of batch entry i, whose kv_rows rows are k_batch_stride apart.
+ * With `causal`, query i of a sequence sees keys j <= i + (keys - queries): aligned to the
+ * last key. key_mask (kv_rows bytes, may be NULL): keys with 0 are not seen, whatever K and V
+ * hold there. bias (may be NULL; uniform only, heads == kv_heads, q_len x kv_len rows): one per
+ * run of bias_seqs consecutive sequences and head.
+ * Strides are in elements, multiples of 8; pointers 16-byte aligned; the head dimension is
+ * contiguous, a multiple of 8, at most 128. out is contiguous (q_rows, heads, head_dim). */
+typedef struct {
+  int32_t dtype, heads, kv_heads, head_dim, causal;
+  float scale; /* finite, >= 0 */
+  int32_t sequences, q_len, kv_len;
+  int64_t q_rows, kv_rows;
+  const int32_t *cu_q, *cu_k, *kv_lengths;
+  const void* q;
+  int64_t q_row_stride, q_head_stride;
+  const void* k;
+  int64_t k_row_stride, k_head_stride, k_batch_stride;
+  const void* v;
+  int64_t v_row_stride, v_head_stride, v_batch_stride;
+  const uint8_t* key_mask;
+  const void* bias;
+  int32_t bias_seqs;
+  int64_t bias_row_stride, bias_head_stride, bias_batch_stride;
+  void* out;
+  float* stats; /* forward: NULL if no backward follows; 2 * q_rows * heads floats */
+} ftm_attention;
+/* Scratch of a forward (0: none needed, or bad arguments). With `train`, a packed call also
+ * leaves there what its backward reads. */
+size_t ftm_attention_workspace_bytes(const ftm_attention* p, int32_t train);
+int ftm_attention_fwd(const ftm_attention* p, int32_t train, void* workspace, size_t workspace_bytes,
+                      int* err_word, ftm_stream_t stream);
+
+/* Backward (not of the cache form): p as in the forward, with its out and stats, and the
+ * forward's workspace (train = 1). grad: (q_rows, heads, head_dim), its strides in elements.
+ * dq like out; dk, dv contiguous (kv_rows, kv_heads, head_dim); dbias contiguous
+ * (sequences / bias_seqs, heads, q_len, kv_len). dq, the pair dk / dv, and dbias may each be
+ * NULL when not wanted, but not all. No atomics: the same bits on every call. */
+size_t ftm_attention_bwd_workspace_bytes(const ftm_attention* p, int32_t want_dbias);
+int ftm_attention_bwd(const ftm_attention* p, const void* grad, int64_t grad_row_stride,
+                      int64_t grad_head_stride, void* fwd_workspace, size_t fwd_workspace_bytes,
+                      void* workspace, size_t workspace_bytes, void* dq, void* dk, void* dv, void* dbias,
+                      int* err_word, ftm_stream_t stream);
+
 /* ---- status -------------------------------------------------------------- */
 /* Synchronise `stream`, read the device error word of a workspace (or any err_word
  * passed to a stage) and clear it: FTM_OK, or FTM_TIMEOUT when a bounded device wait
