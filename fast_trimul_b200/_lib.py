@@ -142,9 +142,9 @@ SIGNATURES = {
     "ftm_layer_norm_bwd": (ctypes.c_int, [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp,
                                           _i32, _vp, _sz, _i64, _i32, _vp]),
     "ftm_attention_workspace_bytes": (_sz, [_PA, _i32]),
-    "ftm_attention_fwd": (ctypes.c_int, [_PA, _i32, _vp, _sz, _vp, _vp]),
+    "ftm_attention_fwd": (ctypes.c_int, [_PA, _i32, _vp, _sz, _vp, _vp, _vp]),
     "ftm_attention_bwd_workspace_bytes": (_sz, [_PA, _i32]),
-    "ftm_attention_bwd": (ctypes.c_int, [_PA, _vp, _i64, _i64, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ftm_attention_bwd": (ctypes.c_int, [_PA, _vp, _i64, _i64, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
 

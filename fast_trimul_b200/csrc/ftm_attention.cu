@@ -195,6 +195,10 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           const uint32_t ph = ((kn / NS) & 1) ^ 1;
           ok = mbar_wait(&k_empty[s], ph, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 2));
           if (!ok) break;
+          if (a.test_stall && kn == 0) {   // nobody can go on: every wait of the block expires
+            ok = false;
+            break;
+          }
           mbar_arrive_expect_tx(&k_full[s], C::kTile);
           load_tile4<DP>(&maps.k, &k_full[s], sK + s * C::kTile, it.head, it.k0 + t * kTileRows, it.kb);
           if (BIAS) {
@@ -218,6 +222,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       }
       ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
     }
+    if (!ok) report_failure(a);
     if (lane == 0) {   // copies in flight land before the block may exit
       if (qn) mbar_wait_drain(q_full, (qn - 1) & 1);
       for (int i = kn > NS ? kn - NS : 0; i < kn; ++i) {
@@ -286,6 +291,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       kn += n;
       ++qn;
     }
+    if (!ok) report_failure(a);
     if (lane == 0) {
       umma_commit(drain);
       mbar_wait_drain(drain, 0);

@@ -50,8 +50,20 @@ struct AttnArgs {
   void* dv;
   void* dbias;
   float* dbias_part;
-  int* err;
+  int* err;                  // device error word the waits poll
+  int* host_err;             // pinned host word that learns of an expired wait; may be null
+  int test_stall;            // withhold the first K tile (failure tests)
 };
+
+// a role that gave up tells the host: polling a host word in the waits themselves would cross
+// PCIe on every poll (measured: 50x slower kernels), so only this write goes there
+__device__ __forceinline__ void report_failure(const AttnArgs& a) {
+  if (a.host_err) {
+    const int code = *reinterpret_cast<volatile int*>(a.err);
+    if (code) *reinterpret_cast<volatile int*>(a.host_err) = code;
+    __threadfence_system();
+  }
+}
 
 struct Item {
   int seq, head;      // sequence, key / value head

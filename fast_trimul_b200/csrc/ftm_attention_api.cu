@@ -1,6 +1,8 @@
 // C entry points of attention (declared in include/fast_trimul_b200.h): argument checks,
 // tensor maps, workspaces and the launch sequences.
 #include <cmath>
+#include <cstdlib>
+#include <cstring>
 
 #include "ftm_attention.cuh"
 
@@ -147,7 +149,7 @@ BwdSpace bwd_space(const ftm_attention* p, int want_dbias, int sms) {
 }
 
 // everything of a launch that does not depend on the pass
-bool fill(AttnLaunch& l, const ftm_attention* p, int dev, int* err, ftm_stream_t stream) {
+bool fill(AttnLaunch& l, const ftm_attention* p, int dev, int* err, int* host_err, ftm_stream_t stream) {
   l.dp = p->head_dim <= 64 ? 64 : 128;
   l.bf16 = p->dtype == FTM_BF16;
   l.bias = p->bias != nullptr;
@@ -180,6 +182,9 @@ bool fill(AttnLaunch& l, const ftm_attention* p, int dev, int* err, ftm_stream_t
   a.out = p->out;
   a.stats = reinterpret_cast<float2*>(p->stats);
   a.err = err;
+  a.host_err = host_err;
+  const char* stall = getenv("FTM_TEST_STALL");
+  a.test_stall = stall && strcmp(stall, "attention") == 0;
   return q_map(&l.m.q, p, p->q, p->q_row_stride, p->q_head_stride) &&
          kv_map(&l.m.k, p, p->k, p->k_row_stride, p->k_head_stride, p->k_batch_stride) &&
          kv_map(&l.m.v, p, p->v, p->v_row_stride, p->v_head_stride, p->v_batch_stride) &&
@@ -201,7 +206,7 @@ size_t ftm_attention_workspace_bytes(const ftm_attention* p, int32_t train) {
 }
 
 int ftm_attention_fwd(const ftm_attention* p, int32_t train, void* workspace, size_t workspace_bytes,
-                      int* err_word, ftm_stream_t stream) {
+                      int* err_word, int* host_word, ftm_stream_t stream) {
   set_last_launch_count(0);
   const int st = check(p);
   if (st != FTM_OK) return st;
@@ -212,7 +217,7 @@ int ftm_attention_fwd(const ftm_attention* p, int32_t train, void* workspace, si
   if (w.total && (!workspace || workspace_bytes < w.total)) return FTM_BAD_WORKSPACE;
   if (!aligned(workspace, 256)) return FTM_BAD_ALIGN;
   AttnLaunch l{};
-  if (!fill(l, p, dev, err_word, stream)) return FTM_LAUNCH_FAILED;
+  if (!fill(l, p, dev, err_word, host_word, stream)) return FTM_LAUNCH_FAILED;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   int launches = 1;
   if (l.a.walk == WALK_LIST) {
@@ -250,7 +255,7 @@ size_t ftm_attention_bwd_workspace_bytes(const ftm_attention* p, int32_t want_db
 int ftm_attention_bwd(const ftm_attention* p, const void* grad, int64_t grad_row_stride,
                       int64_t grad_head_stride, void* fwd_workspace, size_t fwd_workspace_bytes,
                       void* workspace, size_t workspace_bytes, void* dq, void* dk, void* dv, void* dbias,
-                      int* err_word, ftm_stream_t stream) {
+                      int* err_word, int* host_word, ftm_stream_t stream) {
   set_last_launch_count(0);
   const int st = check(p);
   if (st != FTM_OK) return st;
@@ -269,7 +274,7 @@ int ftm_attention_bwd(const ftm_attention* p, const void* grad, int64_t grad_row
     return FTM_BAD_WORKSPACE;
   if (!aligned(workspace, 256) || !aligned(fwd_workspace, 256)) return FTM_BAD_ALIGN;
   AttnLaunch l{};
-  if (!fill(l, p, dev, err_word, stream) || !q_map(&l.m.g, p, grad, grad_row_stride, grad_head_stride))
+  if (!fill(l, p, dev, err_word, host_word, stream) || !q_map(&l.m.g, p, grad, grad_row_stride, grad_head_stride))
     return FTM_LAUNCH_FAILED;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   l.a.o = p->out;

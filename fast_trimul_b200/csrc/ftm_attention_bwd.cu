@@ -266,6 +266,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       }
       ++qn;
     }
+    if (!ok) report_failure(a);
     if (lane == 0) {
       umma_commit(drain);
       mbar_wait_drain(drain, 0);
@@ -588,6 +589,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       }
       qn += tiles;
     }
+    if (!ok) report_failure(a);
     if (lane == 0) {
       umma_commit(drain);
       mbar_wait_drain(drain, 0);
@@ -834,6 +836,7 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
           umma_commit(&empty[s]);
         }
       }
+      if (!ok) report_failure(a);
       umma_commit(drain);
       mbar_wait_drain(drain, 0);
     }

@@ -28,26 +28,30 @@ from .norm import device_guard
 _DT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
-class HostErrorWord:
-    """The error word of the attention kernels of one GPU, in pinned host memory that the
-    kernels write directly: the next call (or `check`) sees an expired wait with a plain read,
-    and no call has to copy anything."""
+class AttentionErrorWord:
+    """The error words of the attention kernels of one GPU: one on the device, which their waits
+    poll, and one in pinned host memory, which a kernel writes only when a wait expired. The
+    next call (or `check`) sees that with a plain read; no call copies or synchronises."""
 
-    def __init__(self):
+    def __init__(self, device):
+        self.dev = torch.zeros(64, dtype=torch.int32, device=device)
         self.host = torch.zeros(16, dtype=torch.int32).pin_memory()
-        self.ptr = self.host.data_ptr()
-        self.word = ctypes.c_int32.from_address(self.ptr)
+        self.ptr, self.host_ptr = self.dev.data_ptr(), self.host.data_ptr()
+        self.word = ctypes.c_int32.from_address(self.host_ptr)
 
     def poll(self):
         code = self.word.value
         if code:
-            self.word.value = 0
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.synchronize(self.dev.device)   # its kernels have drained
+                self.dev.zero_()
+                self.word.value = 0
             raise _lib.NativeKernelError(
                 f"a bounded device wait expired in a native attention kernel (code 0x{code:x}: kernel "
                 f"{code >> 8}, role {(code >> 4) & 15}, site {code & 15}); its output is invalid")
 
     def check(self):
-        torch.cuda.synchronize()
+        torch.cuda.synchronize(self.dev.device)
         self.poll()
 
 
@@ -55,11 +59,11 @@ _ERROR_WORDS = {}
 
 
 def attention_error_word(device=None):
-    """The HostErrorWord of a GPU (default: the current one)."""
+    """The AttentionErrorWord of a GPU (default: the current one)."""
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     w = _ERROR_WORDS.get(index)
     if w is None:
-        w = _ERROR_WORDS[index] = HostErrorWord()
+        w = _ERROR_WORDS[index] = AttentionErrorWord(torch.device("cuda", index))
     return w
 
 
@@ -145,7 +149,7 @@ def _launch(call, q, k, v, bias, train):
         prob = call.problem(q, k, v, bias, out, stats)
         nbytes = lib.ftm_attention_workspace_bytes(prob, train)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _lib.check(lib.ftm_attention_fwd(prob, train, _ptr(ws), nbytes, err.ptr,
+        _lib.check(lib.ftm_attention_fwd(prob, train, _ptr(ws), nbytes, err.ptr, err.host_ptr,
                                          torch.cuda.current_stream().cuda_stream), "ftm_attention_fwd")
     _lib.record_launches()
     return out, stats, ws
@@ -187,7 +191,7 @@ class _Attention(torch.autograd.Function):
             _lib.check(lib.ftm_attention_bwd(
                 prob, grad.data_ptr(), grad.stride(0), grad.stride(1), _ptr(lists),
                 0 if lists is None else lists.numel(), ws.data_ptr(), nbytes, _ptr(dq), _ptr(dk), _ptr(dv),
-                _ptr(db), err.ptr, torch.cuda.current_stream().cuda_stream), "ftm_attention_bwd")
+                _ptr(db), err.ptr, err.host_ptr, torch.cuda.current_stream().cuda_stream), "ftm_attention_bwd")
         _lib.record_launches()
         return dq, dk if need_k else None, dv if need_v else None, db, None
 

@@ -387,10 +387,12 @@ typedef struct {
   float* stats; /* forward: NULL if no backward follows; 2 * q_rows * heads floats */
 } ftm_attention;
 /* Scratch of a forward (0: none needed, or bad arguments). With `train`, a packed call also
- * leaves there what its backward reads. */
+ * leaves there what its backward reads. err_word: a zeroed device word, as in the stages;
+ * host_word (may be NULL): a word of pinned host memory that is written, too, when a bounded
+ * wait expired, so a host can look without a copy. */
 size_t ftm_attention_workspace_bytes(const ftm_attention* p, int32_t train);
 int ftm_attention_fwd(const ftm_attention* p, int32_t train, void* workspace, size_t workspace_bytes,
-                      int* err_word, ftm_stream_t stream);
+                      int* err_word, int* host_word, ftm_stream_t stream);
 
 /* Backward (not of the cache form): p as in the forward, with its out and stats, and the
  * forward's workspace (train = 1). grad: (q_rows, heads, head_dim), its strides in elements.
@@ -401,7 +403,7 @@ size_t ftm_attention_bwd_workspace_bytes(const ftm_attention* p, int32_t want_db
 int ftm_attention_bwd(const ftm_attention* p, const void* grad, int64_t grad_row_stride,
                       int64_t grad_head_stride, void* fwd_workspace, size_t fwd_workspace_bytes,
                       void* workspace, size_t workspace_bytes, void* dq, void* dk, void* dv, void* dbias,
-                      int* err_word, ftm_stream_t stream);
+                      int* err_word, int* host_word, ftm_stream_t stream);
 
 /* ---- status -------------------------------------------------------------- */
 /* Synchronise `stream`, read the device error word of a workspace (or any err_word
