@@ -301,7 +301,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     const int row = threadIdx.x;
     const int tok = row / a.group, gi = row - tok * a.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    const float c = BIAS ? kLog2e : a.scale * kLog2e;     // scores to powers of two
+    const float c = BIAS ? kLog2e : log2_scale(a.scale);     // scores to powers of two
     int kn = 0, on = 0;
     T* out = static_cast<T*>(a.out);
     if (a.walk == WALK_LIST) {
@@ -509,7 +509,7 @@ attn_combine_kernel(const __grid_constant__ AttnArgs a, int blocks) {
   const int t0 = before * a.kv_heads + head * tiles, t1 = t0 + tiles;
   const int c0 = t0 / per, c1 = (t1 - 1) / per;
   if (c0 == c1) return;
-  const float c = a.scale * kLog2e;
+  const float c = log2_scale(a.scale);
   float m = -INFINITY;
   for (int b = c0; b <= c1; ++b) {
     const int slot = 2 * b + (b == c0 && t0 != b * per ? 1 : 0);

@@ -267,6 +267,10 @@ __device__ __forceinline__ uint32_t bits_below(int lim, int word) {
   return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
 }
 
+// Factor from scores to powers of two. A scale of 0 becomes the least normal number: finite
+// scores still meet 0, but a masked -inf does not turn into 0 * inf.
+__device__ __forceinline__ float log2_scale(float scale) { return fmaxf(scale * kLog2e, 1.17549435e-38f); }
+
 struct AttnMaps {
   CUtensorMap q, k, v, g, bias;
 };

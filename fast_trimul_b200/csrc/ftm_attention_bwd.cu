@@ -36,7 +36,7 @@ attn_delta_kernel(const __grid_constant__ AttnArgs a, int lanes, int bias) {
   grid_dep_wait();
   const long long n = static_cast<long long>(a.q_rows) * a.heads;
   const int per = blockDim.x / lanes, l = threadIdx.x % lanes;
-  const float c = a.scale * kLog2e;
+  const float c = log2_scale(a.scale);
   // the bound is the same for all threads of a warp: the sums below exchange lanes
   for (long long i0 = static_cast<long long>(blockIdx.x) * per; i0 < n; i0 += static_cast<long long>(gridDim.x) * per) {
     const long long i = i0 + threadIdx.x / lanes;
@@ -276,7 +276,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
     const int row = quad * 32 + lane;
     const int tok = row / a.group, gi = row - tok * a.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const float c = a.scale * kLog2e;
+    const float c = log2_scale(a.scale);
     T* dq = static_cast<T*>(a.dq);
     if (a.walk == WALK_LIST)
       zero_outside(a.cu_q, a.seqs, a.q_rows, static_cast<long long>(a.heads) * a.dim / 8, dq, threadIdx.x, 256);
@@ -598,7 +598,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     const int quad = warp & 3, half = warp >> 2;
     const int row = quad * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const float c = a.scale * kLog2e;
+    const float c = log2_scale(a.scale);
     T *dk = static_cast<T*>(a.dk), *dv = static_cast<T*>(a.dv);
     if (a.walk == WALK_LIST) {
       const long long per = static_cast<long long>(a.kv_heads) * a.dim / 8;

@@ -13,11 +13,23 @@ The triangle multiplication slots take either `TriMulTorch` (a plain PyTorch Tri
 the role the library's own layer plays) or fast_trimul_b200's
 `FastTriangleMultiplication(residual=False)` -- the only layers that differ between
 the two trunks, as in the reference's trunk comparison. Weights are random.
+
+`fused=True` gives a trunk the library's other operators too: every layer norm is
+`FastLayerNorm` and both attentions run `pair_attention` (fp16 / bf16 on a GPU). Same parameters
+and state dict; the result differs by rounding, and at positions whose mask leaves them no
+key, which the kernels give zeros.
 """
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from .ops.attention import pair_attention
+from .ops.norm import FastLayerNorm
+
+
+def _norm(width, fused):
+    return FastLayerNorm(width) if fused else nn.LayerNorm(width)
 
 
 class TriMulTorch(nn.Module):
@@ -57,10 +69,10 @@ class TriangleAttention(nn.Module):
     """Gated triangle self-attention around the starting (rows) or ending (columns)
     node, with the pair representation as attention bias."""
 
-    def __init__(self, c_z, heads=4, head_dim=32, ending=False):
+    def __init__(self, c_z, heads=4, head_dim=32, ending=False, fused=False):
         super().__init__()
-        self.h, self.d, self.ending = heads, head_dim, ending
-        self.norm = nn.LayerNorm(c_z)
+        self.h, self.d, self.ending, self.fused = heads, head_dim, ending, fused
+        self.norm = _norm(c_z, fused)
         self.qkv = nn.Linear(c_z, 3 * heads * head_dim, bias=False)
         self.bias = nn.Linear(c_z, heads, bias=False)
         self.gate = nn.Linear(c_z, heads * head_dim)
@@ -73,6 +85,11 @@ class TriangleAttention(nn.Module):
         zn = self.norm(z)
         q, k, v = self.qkv(zn).view(B, N, N, 3, self.h, self.d).unbind(3)
         bias = self.bias(zn).permute(0, 3, 1, 2)                    # (B, H, N_j, N_k)
+        if self.fused:
+            m = None if mask is None else (mask.transpose(1, 2) if self.ending else mask) >= 1
+            o = pair_attention(q, k, v, bias, m).reshape(B, N, N, self.h * self.d)
+            o = self.out(torch.sigmoid(self.gate(zn)) * o)
+            return o.transpose(1, 2) if self.ending else o
         q, k, v = (t.permute(0, 1, 3, 2, 4).reshape(B * N, self.h, N, self.d) for t in (q, k, v))
         attn_bias = bias.unsqueeze(1).expand(B, N, self.h, N, N).reshape(B * N, self.h, N, N)
         if mask is not None:
@@ -85,9 +102,9 @@ class TriangleAttention(nn.Module):
 
 
 class SwiGLUTransition(nn.Module):
-    def __init__(self, c, n=4):
+    def __init__(self, c, n=4, fused=False):
         super().__init__()
-        self.norm = nn.LayerNorm(c)
+        self.norm = _norm(c, fused)
         self.up = nn.Linear(c, 2 * n * c, bias=False)
         self.down = nn.Linear(n * c, c, bias=False)
 
@@ -97,11 +114,11 @@ class SwiGLUTransition(nn.Module):
 
 
 class AttentionWithPairBias(nn.Module):
-    def __init__(self, c_s, c_z, heads=16):
+    def __init__(self, c_s, c_z, heads=16, fused=False):
         super().__init__()
-        self.h, self.d = heads, c_s // heads
-        self.norm_s = nn.LayerNorm(c_s)
-        self.norm_z = nn.LayerNorm(c_z)
+        self.h, self.d, self.fused = heads, c_s // heads, fused
+        self.norm_s = _norm(c_s, fused)
+        self.norm_z = _norm(c_z, fused)
         self.qkv = nn.Linear(c_s, 3 * c_s)
         self.bias = nn.Linear(c_z, heads, bias=False)
         self.gate = nn.Linear(c_s, c_s)
@@ -110,23 +127,27 @@ class AttentionWithPairBias(nn.Module):
     def forward(self, s, z):
         B, N, C = s.shape
         sn = self.norm_s(s)
-        q, k, v = self.qkv(sn).view(B, N, 3, self.h, self.d).permute(2, 0, 3, 1, 4)
         bias = self.bias(self.norm_z(z)).permute(0, 3, 1, 2)        # (B, H, N, N)
+        if self.fused:
+            q, k, v = self.qkv(sn).view(B, 1, N, 3, self.h, self.d).unbind(3)
+            o = pair_attention(q, k, v, bias).reshape(B, N, C)
+            return self.out(torch.sigmoid(self.gate(sn)) * o)
+        q, k, v = self.qkv(sn).view(B, N, 3, self.h, self.d).permute(2, 0, 3, 1, 4)
         o = F.scaled_dot_product_attention(q, k, v, attn_mask=bias)
         o = o.transpose(1, 2).reshape(B, N, C)
         return self.out(torch.sigmoid(self.gate(sn)) * o)
 
 
 class PairFormerBlock(nn.Module):
-    def __init__(self, c_s, c_z, trimul_factory, pair_heads=4, pair_head_dim=32):
+    def __init__(self, c_s, c_z, trimul_factory, pair_heads=4, pair_head_dim=32, fused=False):
         super().__init__()
         self.tri_out = trimul_factory(c_z, "outgoing")
         self.tri_in = trimul_factory(c_z, "incoming")
-        self.att_start = TriangleAttention(c_z, pair_heads, pair_head_dim, ending=False)
-        self.att_end = TriangleAttention(c_z, pair_heads, pair_head_dim, ending=True)
-        self.pair_transition = SwiGLUTransition(c_z, 4)
-        self.single_att = AttentionWithPairBias(c_s, c_z)
-        self.single_transition = SwiGLUTransition(c_s, 4)
+        self.att_start = TriangleAttention(c_z, pair_heads, pair_head_dim, ending=False, fused=fused)
+        self.att_end = TriangleAttention(c_z, pair_heads, pair_head_dim, ending=True, fused=fused)
+        self.pair_transition = SwiGLUTransition(c_z, 4, fused=fused)
+        self.single_att = AttentionWithPairBias(c_s, c_z, fused=fused)
+        self.single_transition = SwiGLUTransition(c_s, 4, fused=fused)
 
     def forward(self, s, z, pair_mask=None):
         z = z + self.tri_out(z, mask=pair_mask)
@@ -149,11 +170,13 @@ def fast_trimul(c_z, mode):
 
 
 class PairFormerTrunk(nn.Module):
-    """`blocks` PairFormer blocks whose TriMul layers come from `trimul_factory`."""
+    """`blocks` PairFormer blocks whose TriMul layers come from `trimul_factory`; `fused`: layer
+    norms and attentions on the library's kernels too."""
 
-    def __init__(self, blocks=8, c_s=384, c_z=128, trimul_factory=torch_trimul):
+    def __init__(self, blocks=8, c_s=384, c_z=128, trimul_factory=torch_trimul, fused=False):
         super().__init__()
-        self.blocks = nn.ModuleList(PairFormerBlock(c_s, c_z, trimul_factory) for _ in range(blocks))
+        self.blocks = nn.ModuleList(PairFormerBlock(c_s, c_z, trimul_factory, fused=fused)
+                                    for _ in range(blocks))
 
     def forward(self, s, z, pair_mask=None):
         for blk in self.blocks:
