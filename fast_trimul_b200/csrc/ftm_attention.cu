@@ -34,7 +34,8 @@ struct FwdCfg {
   static constexpr int kOffK = kTile;
   static constexpr int kOffV = kOffK + kStages * kTile;
   static constexpr int kOffB = kOffV + kStages * kTile;
-  static constexpr int kOffBar = kOffB + (BIAS ? 2 * kBlk : 0);
+  static constexpr int kOffM = kOffB + (BIAS ? 2 * kBlk : 0);   // key bits: 2 x 16 bytes
+  static constexpr int kOffBar = kOffM + 32;
   static constexpr int kSmem = kOffBar + 256 + 1024;
 };
 
@@ -120,6 +121,85 @@ struct FwdWalk {
   }
 };
 
+// A row of scores is read twice, 32 columns at a time, the next 32 on their way under these
+// ones' arithmetic: once for the maximum, once for the weights. Held in registers it would
+// spill, and spilled words miss the little L1 that the tiles leave (2 x 8192 tokens, 16 heads
+// of 128: 636 against 842 TFLOP/s). CUT: some keys are not seen; without, no instruction is
+// spent on that (packed arithmetic, 7 instructions for two scores).
+template <bool BIAS, bool CUT, typename T>
+__device__ __forceinline__ float row_max(uint32_t taddr, const uint8_t* sB, int row, float scale, float m,
+                                         const uint32_t (&keep)[4], int lim) {
+  uint32_t r[2][32];
+  float top[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+  FTM_TMEM_LD32_NOWAIT(taddr, r[0]);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t(&x)[32] = r[q & 1];
+    tmem_wait_ld();
+    if (q < 3) FTM_TMEM_LD32_NOWAIT(taddr + (q + 1) * 32, r[(q + 1) & 1]);
+    if (BIAS) {   // scores with the bias go back over the plain ones
+#pragma unroll
+      for (int e8 = 0; e8 < 4; ++e8) {
+        float f[8];
+        unpack8(*reinterpret_cast<const uint4*>(sB + (q >> 1) * kBlk + sw128_off(row, (q & 1) * 4 + e8)),
+                IsBf16<T>::v, f);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const int i = e8 * 8 + e;
+          const float2 t = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])),
+                                      make_float2(scale, scale), make_float2(f[e], f[e + 1]));
+          x[i] = __float_as_uint(t.x);
+          x[i + 1] = __float_as_uint(t.y);
+        }
+      }
+      tmem_st32(taddr + q * 32, x);
+    }
+    if (CUT) {
+      const uint32_t bits = keep[q] & bits_below(lim, q);
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if ((bits >> e) & 1u) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(x[e]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; e += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          top[k] = fmaxf(fmaxf(top[k], __uint_as_float(x[e + k])), __uint_as_float(x[e + k + 4]));
+    }
+  }
+  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+
+// weights 2^(c (t - ref)) of a row, written as 16-bit pairs over its first 64 columns; their sum
+template <bool CUT, bool FAR, typename T>
+__device__ __forceinline__ float row_weights(uint32_t taddr, float c, float ref, const uint32_t (&keep)[4],
+                                             int lim) {
+  uint32_t r[2][32];
+  const float nref = -ref * c;
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  FTM_TMEM_LD32_NOWAIT(taddr, r[0]);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t(&x)[32] = r[q & 1];
+    tmem_wait_ld();
+    if (q < 3) FTM_TMEM_LD32_NOWAIT(taddr + (q + 1) * 32, r[(q + 1) & 1]);
+    const uint32_t bits = CUT ? keep[q] & bits_below(lim, q) : 0u;
+    uint32_t pk[16];
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      float2 y = make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+      if (FAR) y = make_float2((y.x - ref) * c, (y.y - ref) * c);
+      else y = __ffma2_rn(y, make_float2(c, c), make_float2(nref, nref));
+      y = make_float2(ex2(y.x), ex2(y.y));
+      if (CUT) y = make_float2((bits >> e) & 1u ? y.x : 0.f, (bits >> (e + 1)) & 1u ? y.y : 0.f);
+      sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], y);
+      pk[e >> 1] = pack16<T>(y.x, y.y);
+    }
+    tmem_st16(taddr + q * 16, pk);   // over scores that have been read
+  }
+  return (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
+}
+
 template <int DP, bool BIAS, typename T>
 __global__ void __launch_bounds__(kFwdThreads, 2)
 attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnArgs a) {
@@ -132,6 +212,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   uint8_t* sK = smem + C::kOffK;
   uint8_t* sV = smem + C::kOffV;
   uint8_t* sB = smem + C::kOffB;
+  uint32_t* sM = reinterpret_cast<uint32_t*>(smem + C::kOffM);
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* q_empty = q_full + 1;
   uint64_t* k_full = q_full + 2;
@@ -144,7 +225,9 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   uint64_t* p_ready = s_full + 1;
   uint64_t* o_full = p_ready + 1;
   uint64_t* drain = o_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* m_full = drain + 1;     // 2: key bits of a tile, written by the TMA warp
+  uint64_t* m_empty = drain + 3;    // 2: read by the softmax warps and the MMA warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 5);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -162,6 +245,10 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     mbar_init(p_ready, 4);
     mbar_init(o_full, 1);
     mbar_init(drain, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&m_full[s], 1);
+      mbar_init(&m_empty[s], 5);
+    }
     fence_mbar_init();
   }
   if (warp == 5) tmem_alloc(tmem_slot, 256);
@@ -179,56 +266,66 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   if (warp == 4) {
     // ------------------------------------------------------------------------ TMA
     const uint32_t q_bytes = DP / 64 * 128u * (a.group * a.tq);
-    int qn = 0, kn = 0, bn = 0;
+    int qn = 0, kn = 0, kf = 0, vf = 0, bn = 0;   // items, tiles; loads issued of K, V, bias
     bool ok = true;
     while (ok && walk.next(a, it)) {
       if (it.kt1 <= it.kt0) continue;
+      ok = mbar_wait_warp(q_empty, (qn & 1) ^ 1, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 1));
+      if (!ok) break;
       if (lane == 0) {
-        ok = mbar_wait(q_empty, (qn & 1) ^ 1, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 1));
-        if (ok) {
-          mbar_arrive_expect_tx(q_full, q_bytes);
-          load_tile4<DP>(&maps.q, q_full, sQ, 0, it.head, it.q0);
-          ++qn;
-        }
-        for (int t = it.kt0; ok && t < it.kt1; ++t, ++kn) {
-          const int s = kn % NS;
-          const uint32_t ph = ((kn / NS) & 1) ^ 1;
-          ok = mbar_wait(&k_empty[s], ph, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 2));
-          if (!ok) break;
-          if (a.test_stall && kn == 0) {   // nobody can go on: every wait of the block expires
-            ok = false;
-            break;
-          }
+        mbar_arrive_expect_tx(q_full, q_bytes);
+        load_tile4<DP>(&maps.q, q_full, sQ, 0, it.head, it.q0);
+      }
+      ++qn;
+      for (int t = it.kt0; t < it.kt1; ++t) {
+        const int s = kn % NS;
+        const uint32_t ph = ((kn / NS) & 1) ^ 1;
+        ok = mbar_wait_warp(&k_empty[s], ph, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 2)) &&
+             !(a.test_stall && kn == 0);   // (then every wait of the block expires)
+        if (!ok) break;
+        if (lane == 0) {
           mbar_arrive_expect_tx(&k_full[s], C::kTile);
           load_tile4<DP>(&maps.k, &k_full[s], sK + s * C::kTile, it.head, it.k0 + t * kTileRows, it.kb);
-          if (BIAS) {
-            ok = mbar_wait(b_empty, (bn & 1) ^ 1, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 3));
-            if (ok) {
-              mbar_arrive_expect_tx(b_full, 2 * kBlk);
-              for (int h = 0; h < 2; ++h)
-                tma_load_4d(&maps.bias, b_full, sB + h * kBlk, t * kTileRows + h * 64, it.pos0, it.head,
-                            it.seq / a.bias_seqs);
-              ++bn;
-            }
+        }
+        ++kf;
+        if (a.key_mask) {
+          // here, while the tile before is being worked on: the loads' latency is nobody else's
+          const int mb = kn & 1;
+          uint32_t keep[4];
+          key_bits(a, it, t, lane, keep);
+          ok = mbar_wait_warp(&m_empty[mb], ((kn >> 1) & 1) ^ 1, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 5));
+          if (!ok) break;
+          if (lane == 0) {
+            *reinterpret_cast<uint4*>(sM + mb * 4) = make_uint4(keep[0], keep[1], keep[2], keep[3]);
+            mbar_arrive(&m_full[mb]);
           }
-          ok = ok && mbar_wait(&v_empty[s], ph, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 4));
-          if (!ok) {
-            mbar_wait_drain(&k_full[s], (kn / NS) & 1);   // issued alone: not seen by the drain below
-            break;
+        }
+        if (BIAS) {
+          ok = mbar_wait_warp(b_empty, (kn & 1) ^ 1, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 3));
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(b_full, 2 * kBlk);
+            for (int h = 0; h < 2; ++h)
+              tma_load_4d(&maps.bias, b_full, sB + h * kBlk, t * kTileRows + h * 64, it.pos0, it.head,
+                          it.seq / a.bias_seqs);
           }
+          ++bn;
+        }
+        ok = mbar_wait_warp(&v_empty[s], ph, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 4));
+        if (!ok) break;
+        if (lane == 0) {
           mbar_arrive_expect_tx(&v_full[s], C::kTile);
           load_tile4<DP>(&maps.v, &v_full[s], sV + s * C::kTile, it.head, it.k0 + t * kTileRows, it.kb);
         }
+        ++vf;
+        ++kn;
       }
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
     }
     if (!ok) report_failure(a);
     if (lane == 0) {   // copies in flight land before the block may exit
       if (qn) mbar_wait_drain(q_full, (qn - 1) & 1);
-      for (int i = kn > NS ? kn - NS : 0; i < kn; ++i) {
-        mbar_wait_drain(&k_full[i % NS], (i / NS) & 1);
-        mbar_wait_drain(&v_full[i % NS], (i / NS) & 1);
-      }
+      for (int i = kf > NS ? kf - NS : 0; i < kf; ++i) mbar_wait_drain(&k_full[i % NS], (i / NS) & 1);
+      for (int i = vf > NS ? vf - NS : 0; i < vf; ++i) mbar_wait_drain(&v_full[i % NS], (i / NS) & 1);
       if (bn) mbar_wait_drain(b_full, (bn - 1) & 1);
     }
   } else if (warp == 5) {
@@ -248,12 +345,16 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         if (j > 0) {
           const int kj = kn + j - 1, s = kj % NS;
           const int kt = it.kt0 + j - 1;
-          uint32_t keep[4];
-          if (a.key_mask) key_bits(a, it, kt, lane, keep);
           ok = mbar_wait_warp(&v_full[s], (kj / NS) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 2));
+          if (ok && a.key_mask)
+            ok = mbar_wait_warp(&m_full[kj & 1], (kj >> 1) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 5));
           if (!ok) break;
           const int valid = it.klen - kt * kTileRows;
           if (a.key_mask) {
+            const uint4 w = *reinterpret_cast<const uint4*>(sM + (kj & 1) * 4);
+            const uint32_t keep[4] = {w.x, w.y, w.z, w.w};
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&m_empty[kj & 1]);
             if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
               zero_rows_masked<DP>(sV + s * C::kTile, keep, lane);
               fence_proxy_async_smem();
@@ -323,7 +424,12 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         const int lim = seen - kt * kTileRows;
         bool cut = lim < kTileRows;
         if (a.key_mask) {
-          key_bits(a, it, kt, lane, keep);
+          ok = mbar_wait_warp(&m_full[kn & 1], (kn >> 1) & 1, a.err, err_code(KERNEL_ATTN, ROLE_EPILOGUE, 4));
+          if (!ok) break;
+          const uint4 w = *reinterpret_cast<const uint4*>(sM + (kn & 1) * 4);
+          keep[0] = w.x; keep[1] = w.y; keep[2] = w.z; keep[3] = w.w;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&m_empty[kn & 1]);
           cut = cut || (keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu;
         } else {
           keep[0] = keep[1] = keep[2] = keep[3] = 0xffffffffu;
@@ -336,47 +442,14 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         ok = mbar_wait_warp(s_full, kn & 1, a.err, err_code(KERNEL_ATTN, ROLE_EPILOGUE, 2));
         if (!ok) break;
         tc_fence_after();
-        // The row is read twice, 32 columns at a time, the next 32 on their way under this
-        // ones' arithmetic: once for the maximum, once for the weights. Held in registers it
-        // would spill, and spilled words miss the little L1 that the tiles leave (measured at
-        // dim 128: 636 TFLOP/s with 90 spill accesses per row and tile).
-        uint32_t r[2][32];
-        float top[4] = {m, -INFINITY, -INFINITY, -INFINITY};
-        FTM_TMEM_LD32_NOWAIT(lanes, r[0]);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t(&x)[32] = r[q & 1];
-          tmem_wait_ld();
-          if (q < 3) FTM_TMEM_LD32_NOWAIT(lanes + (q + 1) * 32, r[(q + 1) & 1]);
-          if (BIAS) {   // scores with the bias go back over the plain ones
-#pragma unroll
-            for (int e8 = 0; e8 < 4; ++e8) {
-              float f[8];
-              unpack8(*reinterpret_cast<const uint4*>(sB + (q >> 1) * kBlk + sw128_off(row, (q & 1) * 4 + e8)),
-                      IsBf16<T>::v, f);
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                x[e8 * 8 + e] = __float_as_uint(fmaf(__uint_as_float(x[e8 * 8 + e]), a.scale, f[e]));
-            }
-            tmem_st32(lanes + q * 32, x);
-          }
-          if (cut) {
-            const uint32_t bits = keep[q] & bits_below(lim, q);
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if ((bits >> e) & 1u) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(x[e]));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(x[e]));
-          }
-        }
+        float mt;
+        if (cut) mt = row_max<BIAS, true, T>(lanes, sB, row, a.scale, m, keep, lim);
+        else mt = row_max<BIAS, false, T>(lanes, sB, row, a.scale, m, keep, lim);
         if (BIAS) {
           tmem_wait_st();
           __syncwarp();
           if (lane == 0) mbar_arrive(b_empty);
         }
-        FTM_TMEM_LD32_NOWAIT(lanes, r[0]);
-        const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         // keep the old maximum as the reference while it is within 2^8 of the new one
         const bool grow = (mt - m) * c > 8.f || (m == -INFINITY && mt > m);
         if (__any_sync(0xffffffffu, grow)) {
@@ -386,42 +459,24 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             l *= f;
           }
           if (kt > it.kt0) {
-#pragma unroll
-            for (int q = 0; q < DP / 32; ++q) {
-              FTM_TMEM_LD32_NOWAIT(lanes + 128 + q * 32, r[1]);
+#pragma unroll 1
+            for (int q = 0; q * 32 < a.dim; ++q) {
+              uint32_t o[32];
+              FTM_TMEM_LD32_NOWAIT(lanes + 128 + q * 32, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) r[1][e] = __float_as_uint(__uint_as_float(r[1][e]) * f);
-              tmem_st32(lanes + 128 + q * 32, r[1]);
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(lanes + 128 + q * 32, o);
             }
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        const float nref = BIAS ? ref : -ref * c;
-        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t(&x)[32] = r[q & 1];
-          tmem_wait_ld();
-          if (q < 3) FTM_TMEM_LD32_NOWAIT(lanes + (q + 1) * 32, r[(q + 1) & 1]);
-          const uint32_t bits = cut ? keep[q] & bits_below(lim, q) : 0xffffffffu;
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float2 y = make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-            if (BIAS) {   // the difference first: scores near the type's lowest value stay exact
-              y = make_float2((y.x - nref) * c, (y.y - nref) * c);
-            } else {
-              y = __ffma2_rn(y, make_float2(c, c), make_float2(nref, nref));
-            }
-            y = make_float2(ex2(y.x), ex2(y.y));
-            if (cut) y = make_float2((bits >> e) & 1u ? y.x : 0.f, (bits >> (e + 1)) & 1u ? y.y : 0.f);
-            sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], y);
-            pk[e >> 1] = pack16<T>(y.x, y.y);
-          }
-          tmem_st16(lanes + q * 16, pk);   // over scores that have been read
-        }
-        l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
+        // c t - c ref in one rounding, unless a bias has put the whole row far from 0 (down to
+        // the type's lowest value, used as a mask): then the difference first, which is exact
+        const bool far = BIAS && __any_sync(0xffffffffu, fabsf(ref) > 1024.f);
+        if (far) l += row_weights<true, true, T>(lanes, c, ref, keep, lim);
+        else if (cut) l += row_weights<true, false, T>(lanes, c, ref, keep, lim);
+        else l += row_weights<false, false, T>(lanes, c, ref, keep, lim);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -440,6 +495,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
       for (int q = 0; q < DP / 32; ++q) {
+        if (q * 32 >= a.dim) break;
         uint32_t o[32];
         if (any) {
           FTM_TMEM_LD32_NOWAIT(lanes + 128 + q * 32, o);
