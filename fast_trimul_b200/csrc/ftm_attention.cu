@@ -205,6 +205,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
 attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnArgs a) {
   using C = FwdCfg<DP, BIAS>;
   constexpr int NS = C::kStages;
+  constexpr bool E = !(BIAS && DP == 128);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -229,7 +230,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   uint64_t* m_empty = drain + 3;    // 2: read by the softmax warps and the MMA warp
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 5);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform<E>(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
@@ -255,7 +256,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform<E>(*tmem_slot);
   grid_dep_wait();
   grid_dep_release();
 
@@ -368,7 +369,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           ok = mbar_wait_warp(p_ready, kj & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 3));
           if (!ok) break;
           tc_fence_after();
-          if (lane == 0) {
+          if (issuer<E>(lane)) {
             mma_cols(tmem + 128, tmem, smem_u32(sV + s * C::kTile), id_o, j > 1);
             umma_commit(&v_empty[s]);
             if (j == n) umma_commit(o_full);
@@ -380,8 +381,8 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           ok = mbar_wait_warp(&k_full[s], (kj / NS) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 4));
           if (!ok) break;
           tc_fence_after();
-          if (lane == 0) {
-            mma_rows(tmem, q_addr, smem_u32(sK + s * C::kTile), id_s, a.ksteps);
+          if (issuer<E>(lane)) {
+            mma_rows<E>(tmem, q_addr, smem_u32(sK + s * C::kTile), id_s, a.ksteps);
             umma_commit(s_full);
             umma_commit(&k_empty[s]);
             if (j == n - 1) umma_commit(q_empty);
@@ -393,7 +394,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       ++qn;
     }
     if (!ok) report_failure(a);
-    if (lane == 0) {
+    if (issuer<E>(lane)) {
       umma_commit(drain);
       mbar_wait_drain(drain, 0);
     }
@@ -529,8 +530,10 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       tc_fence_before();   // O read before the next item's first P V is released by p_ready
     }
   }
+  __syncwarp();      // the lanes of a role that one lane drained
   __syncthreads();
   tc_fence_after();
+  __syncwarp();
   if (warp == 5) tmem_dealloc(tmem, 256);
 }
 

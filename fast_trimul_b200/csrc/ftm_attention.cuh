@@ -211,12 +211,44 @@ __device__ __forceinline__ float ex2(float x) {
 // Tiles in shared memory: DP / 64 blocks of 128 rows x 128 bytes (128-byte swizzle).
 constexpr int kBlk = kTileRows * 128;   // bytes of one 64-element block
 
-// D[128 x 128] = A[128 rows x dim] B[128 rows x dim]^T, both K-major
-__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int ksteps) {
-  for (int k = 0; k < ksteps; ++k) {
-    const uint32_t o = (k >> 2) * kBlk + (k & 3) * 32;
-    umma_f16(d, kmajor_desc(a + o), kmajor_desc(b + o), idesc, k > 0 ? 1u : 0u);
+// The lane of a converged warp that issues its matrix instructions. These take descriptors
+// from uniform registers. Behind `elect.sync` the compiler keeps the (warp-uniform) operands
+// there; behind `lane == 0` it moves each one over before every instruction: about 120 clocks
+// per issued MMA, 950 for one P V, which bound the whole kernel. The lanes meet first: an
+// election among some of them would pick another lane, whose commits do not cover the MMAs of
+// the first one.
+// E: which of the two. The kernels with a bias at DP = 128 keep lane 0: with the election they
+// ended with an illegal address that neither reading nor checks of every descriptor and TMEM
+// address explained, so they stay in the form that was tested.
+template <bool E>
+__device__ __forceinline__ bool issuer(int lane) {
+  if (!E) return lane == 0;
+  uint32_t p;
+  __syncwarp();
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// a value that is the same in all lanes, where the compiler cannot see that it is
+template <bool E>
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return E ? __shfl_sync(0xffffffffu, x, 0) : x; }
+
+// D[128 x 128] = A[128 rows x dim] B[128 rows x dim]^T, both K-major; `steps` 16-element steps
+template <bool E>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps) {
+  if (!E) {
+    for (int k = 0; k < steps; ++k) {
+      const uint32_t o = (k >> 2) * kBlk + (k & 3) * 32;
+      umma_f16(d, kmajor_desc(a + o), kmajor_desc(b + o), idesc, k > 0 ? 1u : 0u);
+    }
+    return;
   }
+  const uint64_t ad = kmajor_desc(a), bd = kmajor_desc(b);
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (k < steps) {   // descriptor addresses count 16 bytes
+      const uint64_t o = ((k >> 2) * kBlk + (k & 3) * 32) >> 4;
+      umma_f16(d, ad + o, bd + o, idesc, k > 0 ? 1u : 0u);
+    }
 }
 // D[128 x DP] (+)= A[tmem, 128 x 128] B[128 rows x DP], B MN-major
 __device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t idesc,

@@ -115,6 +115,7 @@ template <int DP, bool BIAS, typename T>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnArgs a) {
   using C = DqCfg<DP, BIAS>;
+  constexpr bool E = !(BIAS && DP == 128);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
@@ -137,7 +138,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
   uint64_t* drain = q_full + 17;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 18);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform<E>(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 18; ++i) mbar_init(q_full + i, i == 11 || i == 15 ? 8 : 1);
     fence_mbar_init();
@@ -146,7 +147,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform<E>(*tmem_slot);
   grid_dep_wait();
   grid_dep_release();
   // columns: S of even tiles 0, dP 128, dQ 256, S of odd tiles 384
@@ -223,8 +224,8 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
         __syncwarp();
       }
       tc_fence_after();
-      if (lane == 0) {
-        mma_rows(tmem + (s ? 384 : 0), q_addr, smem_u32(sK + s * C::kTile), id_s, a.ksteps);
+      if (issuer<E>(lane)) {
+        mma_rows<E>(tmem + (s ? 384 : 0), q_addr, smem_u32(sK + s * C::kTile), id_s, a.ksteps);
         umma_commit(&s_full[s]);
       }
       __syncwarp();
@@ -234,8 +235,8 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       const int s = i & 1;
       if (!mbar_wait_warp(&v_full[s], (i >> 1) & 1, a.err, err_code(KERNEL_DQ, ROLE_MMA, 3))) return false;
       tc_fence_after();
-      if (lane == 0) {
-        mma_rows(tmem + 128, g_addr, smem_u32(sV + s * C::kTile), id_s, a.ksteps);
+      if (issuer<E>(lane)) {
+        mma_rows<E>(tmem + 128, g_addr, smem_u32(sV + s * C::kTile), id_s, a.ksteps);
         umma_commit(dp_full);
         umma_commit(&v_empty[s]);
       }
@@ -253,7 +254,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
         if (ok && j + 1 < tiles) ok = weights_grad(kn + 1);
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) {
+        if (issuer<E>(lane)) {
           const int s = kn & 1;
           mma_cols(tmem + 256, tmem + (s ? 384 : 0), smem_u32(sK + s * C::kTile), id_o, j > 0);
           umma_commit(&k_empty[s]);
@@ -267,7 +268,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       ++qn;
     }
     if (!ok) report_failure(a);
-    if (lane == 0) {
+    if (issuer<E>(lane)) {
       umma_commit(drain);
       mbar_wait_drain(drain, 0);
     }
@@ -378,8 +379,10 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       tc_fence_before();
     }
   }
+  __syncwarp();      // the lanes of a role that one lane drained
   __syncthreads();
   tc_fence_after();
+  __syncwarp();
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
@@ -402,6 +405,7 @@ template <int DP, bool BIAS, typename T>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnArgs a) {
   using C = DkvCfg<DP, BIAS>;
+  constexpr bool E = !(BIAS && DP == 128);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sK = smem;
@@ -428,7 +432,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   uint64_t* drain = kv_full + 21;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_full + 22);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform<E>(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 22; ++i)
       mbar_init(kv_full + i, i == 11 || i == 14 || i == 15 || i == 17 || i == 19 ? 8 : 1);
@@ -447,7 +451,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform<E>(*tmem_slot);
   grid_dep_wait();
   grid_dep_release();
   // columns: S^T / P^T 0, dP^T / dS^T 128, dV 256, dK 384
@@ -549,7 +553,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           ok = mbar_wait_warp(p_ready, i & 1, a.err, err_code(KERNEL_DKV, ROLE_MMA, 2));
           if (!ok) break;
           tc_fence_after();
-          if (lane == 0) {
+          if (issuer<E>(lane)) {
             mma_cols(tmem + 256, tmem, smem_u32(sG + s * C::kTile), id_o, j > 0);
             umma_commit(&g_empty[s]);
           }
@@ -558,8 +562,8 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         if (j + 1 < tiles) {   // behind dV in the pipe, so S^T may overwrite P^T
           ok = arrived(q_full, sQ, i + 1, it.kt0 + j + 1, 3);
           if (!ok) break;
-          if (lane == 0) {
-            mma_rows(tmem, k_addr, smem_u32(sQ + ((i + 1) & 1) * C::kTile), id_s, a.ksteps);
+          if (issuer<E>(lane)) {
+            mma_rows<E>(tmem, k_addr, smem_u32(sQ + ((i + 1) & 1) * C::kTile), id_s, a.ksteps);
             umma_commit(s_full);
           }
           __syncwarp();
@@ -568,7 +572,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           ok = mbar_wait_warp(ds_ready, i & 1, a.err, err_code(KERNEL_DKV, ROLE_MMA, 4));
           if (!ok) break;
           tc_fence_after();
-          if (lane == 0) {
+          if (issuer<E>(lane)) {
             mma_cols(tmem + 384, tmem + 128, smem_u32(sQ + s * C::kTile), id_o, j > 0);
             umma_commit(&q_empty[s]);
           }
@@ -577,20 +581,21 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         if (j + 1 < tiles) {
           ok = arrived(g_full, sG, i + 1, it.kt0 + j + 1, 5);
           if (!ok) break;
-          if (lane == 0) {
-            mma_rows(tmem + 128, v_addr, smem_u32(sG + ((i + 1) & 1) * C::kTile), id_s, a.ksteps);
+          if (issuer<E>(lane)) {
+            mma_rows<E>(tmem + 128, v_addr, smem_u32(sG + ((i + 1) & 1) * C::kTile), id_s, a.ksteps);
             umma_commit(dp_full);
           }
           __syncwarp();
-        } else if (lane == 0) {
+        } else if (issuer<E>(lane)) {
           umma_commit(acc_full);
           umma_commit(kv_empty);
         }
+        __syncwarp();
       }
       qn += tiles;
     }
     if (!ok) report_failure(a);
-    if (lane == 0) {
+    if (issuer<E>(lane)) {
       umma_commit(drain);
       mbar_wait_drain(drain, 0);
     }
@@ -726,8 +731,10 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       tc_fence_before();
     }
   }
+  __syncwarp();      // the lanes of a role that one lane drained
   __syncthreads();
   tc_fence_after();
+  __syncwarp();
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
@@ -746,6 +753,7 @@ template <int DP, typename T>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnArgs a) {
   using C = DbCfg<DP>;
+  constexpr bool E = DP == 64;
   constexpr int NS = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -758,7 +766,7 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
   uint64_t* b_empty = full + 9;
   uint64_t* drain = full + 10;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + 11);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform<E>(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 11; ++i) mbar_init(full + i, i == 6 || i == 7 || i == 9 ? 8 : 1);
     fence_mbar_init();
@@ -767,7 +775,7 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform<E>(*tmem_slot);
   grid_dep_wait();
   grid_dep_release();
 
@@ -830,8 +838,8 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
           if (!ok) break;
           tc_fence_after();
           const uint32_t st = smem_u32(smem + s * C::kStage);
-          mma_rows(tmem + tb * 256, st, st + 2 * C::kTile, id_s, a.ksteps);
-          mma_rows(tmem + tb * 256 + 128, st + C::kTile, st + 3 * C::kTile, id_s, a.ksteps);
+          mma_rows<E>(tmem + tb * 256, st, st + 2 * C::kTile, id_s, a.ksteps);
+          mma_rows<E>(tmem + tb * 256 + 128, st + C::kTile, st + 3 * C::kTile, id_s, a.ksteps);
           umma_commit(&t_full[tb]);
           umma_commit(&empty[s]);
         }
@@ -909,8 +917,10 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
       }
     }
   }
+  __syncwarp();      // the lanes of a role that one lane drained
   __syncthreads();
   tc_fence_after();
+  __syncwarp();
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
