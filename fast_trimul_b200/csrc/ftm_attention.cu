@@ -31,6 +31,11 @@ template <int DP, bool BIAS>
 struct FwdCfg {
   static constexpr int kTile = DP / 64 * kBlk;
   static constexpr int kStages = (DP == 64 && !BIAS) ? 2 : 1;   // K and V each
+  // TMEM columns: S 0 - 127, O from 128. At DP = 64 there is room for P behind O, so the next
+  // tile's scores need not wait for P V; at DP = 128 P lies over S.
+  static constexpr bool kOwnP = DP == 64;
+  static constexpr int kUnroll = (DP == 64 && !BIAS) ? 2 : 1;
+  static constexpr int kColP = kOwnP ? 192 : 0;
   static constexpr int kOffK = kTile;
   static constexpr int kOffV = kOffK + kStages * kTile;
   static constexpr int kOffB = kOffV + kStages * kTile;
@@ -124,42 +129,56 @@ struct FwdWalk {
 // A row of scores is read twice, 32 columns at a time, the next 32 on their way under these
 // ones' arithmetic: once for the maximum, once for the weights. Held in registers it would
 // spill, and spilled words miss the little L1 that the tiles leave (2 x 8192 tokens, 16 heads
-// of 128: 636 against 842 TFLOP/s). CUT: some keys are not seen; without, no instruction is
-// spent on that (packed arithmetic, 7 instructions for two scores).
-template <bool BIAS, bool CUT, typename T>
+// of 128: 636 against 842 TFLOP/s). CUT: some keys are not seen, and their scores become -inf in
+// the first pass; without, no instruction is spent on that. UN: halves of the row per step of
+// the loop; 2 where the registers allow it (N = 384, 4 heads of 32 without a bias: 112 against
+// 123 us), 1 with a bias (147 against 194 us, whose spills came back from L2).
+template <bool BIAS, bool CUT, int UN, typename T>
 __device__ __forceinline__ float row_max(uint32_t taddr, const uint8_t* sB, int row, float scale, float m,
                                          const uint32_t (&keep)[4], int lim) {
   uint32_t r[2][32];
   float top[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+  uint4 braw[4];   // the next 32 columns of the bias, a step ahead too
+  auto load_bias = [&](int q) {
+    if (BIAS) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        braw[i] = *reinterpret_cast<const uint4*>(sB + (q >> 1) * kBlk + sw128_off(row, (q & 1) * 4 + i));
+    }
+  };
   FTM_TMEM_LD32_NOWAIT(taddr, r[0]);
+  load_bias(0);
+#pragma unroll UN
+  for (int half = 0; half < 2; ++half) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    uint32_t(&x)[32] = r[q & 1];
-    tmem_wait_ld();
-    if (q < 3) FTM_TMEM_LD32_NOWAIT(taddr + (q + 1) * 32, r[(q + 1) & 1]);
-    if (BIAS) {   // scores with the bias go back over the plain ones
+    for (int h = 0; h < 2; ++h) {
+      const int q = half * 2 + h;
+      uint32_t(&x)[32] = r[h];
+      tmem_wait_ld();
+      if (q < 3) FTM_TMEM_LD32_NOWAIT(taddr + (q + 1) * 32, r[h ^ 1]);
+      if (BIAS) {   // scores with the bias go back over the plain ones
 #pragma unroll
-      for (int e8 = 0; e8 < 4; ++e8) {
-        float f[8];
-        unpack8(*reinterpret_cast<const uint4*>(sB + (q >> 1) * kBlk + sw128_off(row, (q & 1) * 4 + e8)),
-                IsBf16<T>::v, f);
+        for (int e8 = 0; e8 < 4; ++e8) {
+          float f[8];
+          unpack8(braw[e8], IsBf16<T>::v, f);
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const int i = e8 * 8 + e;
-          const float2 t = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])),
-                                      make_float2(scale, scale), make_float2(f[e], f[e + 1]));
-          x[i] = __float_as_uint(t.x);
-          x[i + 1] = __float_as_uint(t.y);
+          for (int e = 0; e < 8; e += 2) {
+            const int i = e8 * 8 + e;
+            const float2 t = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])),
+                                        make_float2(scale, scale), make_float2(f[e], f[e + 1]));
+            x[i] = __float_as_uint(t.x);
+            x[i + 1] = __float_as_uint(t.y);
+          }
         }
       }
-      tmem_st32(taddr + q * 32, x);
-    }
-    if (CUT) {
-      const uint32_t bits = keep[q] & bits_below(lim, q);
+      if (CUT) {
+        const uint32_t bits = (half ? keep[2 + h] : keep[h]) & bits_below(lim, q);
 #pragma unroll
-      for (int e = 0; e < 32; ++e)
-        if ((bits >> e) & 1u) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(x[e]));
-    } else {
+        for (int e = 0; e < 32; ++e)
+          if (!(bits & (1u << e))) x[e] = 0xff800000u;   // -inf
+      }
+      if (BIAS || CUT) tmem_st32(taddr + q * 32, x);
+      if (q < 3) load_bias(q + 1);
 #pragma unroll
       for (int e = 0; e < 32; e += 8)
 #pragma unroll
@@ -167,35 +186,42 @@ __device__ __forceinline__ float row_max(uint32_t taddr, const uint8_t* sB, int 
           top[k] = fmaxf(fmaxf(top[k], __uint_as_float(x[e + k])), __uint_as_float(x[e + k + 4]));
     }
   }
+  if (BIAS || CUT) tmem_wait_st();
   return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
 
-// weights 2^(c (t - ref)) of a row, written as 16-bit pairs over its first 64 columns; their sum
-template <bool CUT, bool FAR, typename T>
-__device__ __forceinline__ float row_weights(uint32_t taddr, float c, float ref, const uint32_t (&keep)[4],
-                                             int lim) {
+// Weights 2^(c (t - ref)) of a row, written as 16-bit pairs to 64 columns at `paddr` (which may
+// be the scores' own first columns: those have been read by then); their sum. `before_store`
+// runs in front of the first store. FAR: the difference first (see the call).
+// (A polynomial on the FMA pipe for a fourth to a half of the exponentials measured the same
+// time within 2 %: these loops are bound by latency, not by the special function unit.)
+template <bool FAR, int UN, typename T, typename F>
+__device__ __forceinline__ float row_weights(uint32_t taddr, uint32_t paddr, float c, float ref, F before_store) {
   uint32_t r[2][32];
   const float nref = -ref * c;
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   FTM_TMEM_LD32_NOWAIT(taddr, r[0]);
+#pragma unroll UN
+  for (int half = 0; half < 2; ++half) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    uint32_t(&x)[32] = r[q & 1];
-    tmem_wait_ld();
-    if (q < 3) FTM_TMEM_LD32_NOWAIT(taddr + (q + 1) * 32, r[(q + 1) & 1]);
-    const uint32_t bits = CUT ? keep[q] & bits_below(lim, q) : 0u;
-    uint32_t pk[16];
+    for (int h = 0; h < 2; ++h) {
+      const int q = half * 2 + h;
+      uint32_t(&x)[32] = r[h];
+      tmem_wait_ld();
+      if (q < 3) FTM_TMEM_LD32_NOWAIT(taddr + (q + 1) * 32, r[h ^ 1]);
+      uint32_t pk[16];
 #pragma unroll
-    for (int e = 0; e < 32; e += 2) {
-      float2 y = make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-      if (FAR) y = make_float2((y.x - ref) * c, (y.y - ref) * c);
-      else y = __ffma2_rn(y, make_float2(c, c), make_float2(nref, nref));
-      y = make_float2(ex2(y.x), ex2(y.y));
-      if (CUT) y = make_float2((bits >> e) & 1u ? y.x : 0.f, (bits >> (e + 1)) & 1u ? y.y : 0.f);
-      sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], y);
-      pk[e >> 1] = pack16<T>(y.x, y.y);
+      for (int e = 0; e < 32; e += 2) {
+        float2 y = make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+        if (FAR) y = make_float2((y.x - ref) * c, (y.y - ref) * c);
+        else y = __ffma2_rn(y, make_float2(c, c), make_float2(nref, nref));
+        y = make_float2(ex2(y.x), ex2(y.y));
+        sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], y);
+        pk[e >> 1] = pack16<T>(y.x, y.y);
+      }
+      if (q == 0) before_store();
+      tmem_st16(paddr + q * 16, pk);
     }
-    tmem_st16(taddr + q * 16, pk);   // over scores that have been read
   }
   return (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
 }
@@ -228,7 +254,8 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   uint64_t* drain = o_full + 1;
   uint64_t* m_full = drain + 1;     // 2: key bits of a tile, written by the TMA warp
   uint64_t* m_empty = drain + 3;    // 2: read by the softmax warps and the MMA warp
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 5);
+  uint64_t* pv_done = drain + 5;    // O and P of a tile free again (own P columns only)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 6);
 
   const int warp = uniform<E>(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -246,6 +273,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     mbar_init(p_ready, 4);
     mbar_init(o_full, 1);
     mbar_init(drain, 1);
+    mbar_init(pv_done, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&m_full[s], 1);
       mbar_init(&m_empty[s], 5);
@@ -269,7 +297,20 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     const uint32_t q_bytes = DP / 64 * 128u * (a.group * a.tq);
     int qn = 0, kn = 0, kf = 0, vf = 0, bn = 0;   // items, tiles; loads issued of K, V, bias
     bool ok = true;
-    while (ok && walk.next(a, it)) {
+    Item next;
+    for (bool more = walk.next(a, next); ok && more;) {
+      it = next;
+      more = walk.next(a, next);
+      if (more && next.kt1 > next.kt0 && lane == 0) {
+        // the next item's first tiles on their way to L2: its Q can only be loaded once the
+        // last scores of this one are formed, and from HBM would come too late
+#pragma unroll
+        for (int h = 0; h < DP / 64; ++h) {
+          tma_prefetch_l2_4d(&maps.q, h * 64, 0, next.head, next.q0);
+          tma_prefetch_l2_4d(&maps.k, h * 64, next.head, next.k0 + next.kt0 * kTileRows, next.kb);
+          tma_prefetch_l2_4d(&maps.v, h * 64, next.head, next.k0 + next.kt0 * kTileRows, next.kb);
+        }
+      }
       if (it.kt1 <= it.kt0) continue;
       ok = mbar_wait_warp(q_empty, (qn & 1) ^ 1, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 1));
       if (!ok) break;
@@ -336,58 +377,73 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     const uint32_t q_addr = smem_u32(sQ);
     int qn = 0, kn = 0;        // items with keys; key tiles
     bool ok = true;
-    while (ok && walk.next(a, it)) {
+    Item next;                 // found while this item's tiles are at work
+    for (bool more = walk.next(a, next); ok && more;) {
+      it = next;
       const int n = it.kt1 - it.kt0;
-      if (n <= 0) continue;
+      if (n <= 0) {
+        more = walk.next(a, next);
+        continue;
+      }
       ok = mbar_wait_warp(q_full, qn & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 1));
-      for (int j = 0; ok && j <= n; ++j) {
-        // scores of tile j are issued behind P V of tile j - 1: the tensor pipe runs them
-        // in order, so S may overwrite the P that P V reads
-        if (j > 0) {
-          const int kj = kn + j - 1, s = kj % NS;
-          const int kt = it.kt0 + j - 1;
-          ok = mbar_wait_warp(&v_full[s], (kj / NS) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 2));
-          if (ok && a.key_mask)
-            ok = mbar_wait_warp(&m_full[kj & 1], (kj >> 1) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 5));
-          if (!ok) break;
-          const int valid = it.klen - kt * kTileRows;
-          if (a.key_mask) {
-            const uint4 w = *reinterpret_cast<const uint4*>(sM + (kj & 1) * 4);
-            const uint32_t keep[4] = {w.x, w.y, w.z, w.w};
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&m_empty[kj & 1]);
-            if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
-              zero_rows_masked<DP>(sV + s * C::kTile, keep, lane);
-              fence_proxy_async_smem();
-              __syncwarp();
-            }
-          } else if (valid < kTileRows) {
-            zero_rows_from<DP>(sV + s * C::kTile, valid, lane);
+      auto arrived = [&](int j) -> bool {
+        const int kj = kn + j;
+        return mbar_wait_warp(&k_full[kj % NS], (kj / NS) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 4));
+      };
+      auto scores = [&](int j) {
+        const int s = (kn + j) % NS;
+        tc_fence_after();
+        if (issuer<E>(lane)) {
+          mma_rows<E>(tmem, q_addr, smem_u32(sK + s * C::kTile), id_s, a.ksteps);
+          umma_commit(s_full);
+          umma_commit(&k_empty[s]);
+          if (j == n - 1) umma_commit(q_empty);
+        }
+        __syncwarp();
+      };
+      ok = ok && arrived(0);
+      if (ok) scores(0);
+      more = walk.next(a, next);
+      for (int j = 0; ok && j < n; ++j) {
+        // P V of tile j and the scores of tile j + 1. Where P lies over S the scores come
+        // second (the tensor pipe runs in order), else first: the softmax waits for them.
+        const int kj = kn + j, s = kj % NS;
+        const int kt = it.kt0 + j;
+        ok = mbar_wait_warp(&v_full[s], (kj / NS) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 2));
+        if (ok && a.key_mask)
+          ok = mbar_wait_warp(&m_full[kj & 1], (kj >> 1) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 5));
+        if (!ok) break;
+        const int valid = it.klen - kt * kTileRows;
+        if (a.key_mask) {
+          const uint4 w = *reinterpret_cast<const uint4*>(sM + (kj & 1) * 4);
+          const uint32_t keep[4] = {w.x, w.y, w.z, w.w};
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&m_empty[kj & 1]);
+          if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
+            zero_rows_masked<DP>(sV + s * C::kTile, keep, lane);
             fence_proxy_async_smem();
             __syncwarp();
           }
-          ok = mbar_wait_warp(p_ready, kj & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 3));
-          if (!ok) break;
-          tc_fence_after();
-          if (issuer<E>(lane)) {
-            mma_cols(tmem + 128, tmem, smem_u32(sV + s * C::kTile), id_o, j > 1);
-            umma_commit(&v_empty[s]);
-            if (j == n) umma_commit(o_full);
-          }
+        } else if (valid < kTileRows) {
+          zero_rows_from<DP>(sV + s * C::kTile, valid, lane);
+          fence_proxy_async_smem();
           __syncwarp();
         }
-        if (j < n) {
-          const int kj = kn + j, s = kj % NS;
-          ok = mbar_wait_warp(&k_full[s], (kj / NS) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 4));
-          if (!ok) break;
-          tc_fence_after();
-          if (issuer<E>(lane)) {
-            mma_rows<E>(tmem, q_addr, smem_u32(sK + s * C::kTile), id_s, a.ksteps);
-            umma_commit(s_full);
-            umma_commit(&k_empty[s]);
-            if (j == n - 1) umma_commit(q_empty);
-          }
-          __syncwarp();
+        if (C::kOwnP && j + 1 < n) ok = arrived(j + 1);
+        ok = ok && mbar_wait_warp(p_ready, kj & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 3));
+        if (ok && C::kOwnP && j + 1 < n) scores(j + 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (issuer<E>(lane)) {
+          mma_cols(tmem + 128, tmem + C::kColP, smem_u32(sV + s * C::kTile), id_o, j > 0);
+          umma_commit(&v_empty[s]);
+          if (C::kOwnP) umma_commit(pv_done);
+          if (j + 1 == n) umma_commit(o_full);
+        }
+        __syncwarp();
+        if (!C::kOwnP && j + 1 < n) {
+          ok = arrived(j + 1);
+          if (ok) scores(j + 1);
         }
       }
       kn += n;
@@ -444,13 +500,19 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         if (!ok) break;
         tc_fence_after();
         float mt;
-        if (cut) mt = row_max<BIAS, true, T>(lanes, sB, row, a.scale, m, keep, lim);
-        else mt = row_max<BIAS, false, T>(lanes, sB, row, a.scale, m, keep, lim);
+        if (cut) mt = row_max<BIAS, true, 1, T>(lanes, sB, row, a.scale, m, keep, lim);
+        else mt = row_max<BIAS, false, C::kUnroll, T>(lanes, sB, row, a.scale, m, keep, lim);
         if (BIAS) {
-          tmem_wait_st();
           __syncwarp();
           if (lane == 0) mbar_arrive(b_empty);
         }
+        // P V of the tile before has read P and written O
+        auto pv_wait = [&] {
+          if (C::kOwnP && kn > 0) {
+            ok = ok && mbar_wait_warp(pv_done, (kn - 1) & 1, a.err, err_code(KERNEL_ATTN, ROLE_EPILOGUE, 5));
+            tc_fence_after();
+          }
+        };
         // keep the old maximum as the reference while it is within 2^8 of the new one
         const bool grow = (mt - m) * c > 8.f || (m == -INFINITY && mt > m);
         if (__any_sync(0xffffffffu, grow)) {
@@ -460,6 +522,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             l *= f;
           }
           if (kt > it.kt0) {
+            pv_wait();
 #pragma unroll 1
             for (int q = 0; q * 32 < a.dim; ++q) {
               uint32_t o[32];
@@ -475,9 +538,9 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         // c t - c ref in one rounding, unless a bias has put the whole row far from 0 (down to
         // the type's lowest value, used as a mask): then the difference first, which is exact
         const bool far = BIAS && __any_sync(0xffffffffu, fabsf(ref) > 1024.f);
-        if (far) l += row_weights<true, true, T>(lanes, c, ref, keep, lim);
-        else if (cut) l += row_weights<true, false, T>(lanes, c, ref, keep, lim);
-        else l += row_weights<false, false, T>(lanes, c, ref, keep, lim);
+        if (far) l += row_weights<true, 1, T>(lanes, lanes + C::kColP, c, ref, pv_wait);
+        else l += row_weights<false, C::kUnroll, T>(lanes, lanes + C::kColP, c, ref, pv_wait);
+        if (!ok) break;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -494,9 +557,8 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       const int head = it.head * a.group + gi;
       const size_t orow = (static_cast<size_t>(it.q0) + tok) * a.heads + head;
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-#pragma unroll
-      for (int q = 0; q < DP / 32; ++q) {
-        if (q * 32 >= a.dim) break;
+#pragma unroll 1
+      for (int q = 0; q * 32 < a.dim; ++q) {
         uint32_t o[32];
         if (any) {
           FTM_TMEM_LD32_NOWAIT(lanes + 128 + q * 32, o);

@@ -274,17 +274,18 @@ __device__ __forceinline__ void zero_rows_from(uint8_t* tile, int first, int lan
     for (int i = first * 8 + lane; i < kTileRows * 8; i += 32)
       reinterpret_cast<uint4*>(tile + h * kBlk)[i] = make_uint4(0, 0, 0, 0);
 }
-// the same for the rows whose bit is clear
+// the same for the rows whose bit is clear: 32 rows at a time, DP / 8 lanes a row
 template <int DP>
 __device__ __forceinline__ void zero_rows_masked(uint8_t* tile, const uint32_t (&keep)[4], int lane) {
+  constexpr int kLanes = DP / 8, kRows = 32 / kLanes;
+  const int l = lane % kLanes;
+  uint8_t* at = tile + (l >> 3) * kBlk + (l & 7) * 16;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    for (uint32_t gone = ~keep[w]; gone; gone &= gone - 1) {
-      const int r = w * 32 + __ffs(gone) - 1;
-      if (lane < DP / 8)
-        *reinterpret_cast<uint4*>(tile + (lane >> 3) * kBlk + r * 128 + (lane & 7) * 16) =
-            make_uint4(0, 0, 0, 0);
-    }
+    if (keep[w] == 0xffffffffu) continue;
+#pragma unroll 4
+    for (int i = lane / kLanes; i < 32; i += kRows)
+      if (!((keep[w] >> i) & 1u)) *reinterpret_cast<uint4*>(at + (w * 32 + i) * 128) = make_uint4(0, 0, 0, 0);
   }
 }
 
