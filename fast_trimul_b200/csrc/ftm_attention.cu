@@ -138,16 +138,7 @@ __device__ __forceinline__ float row_max(uint32_t taddr, const uint8_t* sB, int 
                                          const uint32_t (&keep)[4], int lim) {
   uint32_t r[2][32];
   float top[4] = {m, -INFINITY, -INFINITY, -INFINITY};
-  uint4 braw[4];   // the next 32 columns of the bias, a step ahead too
-  auto load_bias = [&](int q) {
-    if (BIAS) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        braw[i] = *reinterpret_cast<const uint4*>(sB + (q >> 1) * kBlk + sw128_off(row, (q & 1) * 4 + i));
-    }
-  };
   FTM_TMEM_LD32_NOWAIT(taddr, r[0]);
-  load_bias(0);
 #pragma unroll UN
   for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -159,13 +150,13 @@ __device__ __forceinline__ float row_max(uint32_t taddr, const uint8_t* sB, int 
       if (BIAS) {   // scores with the bias go back over the plain ones
 #pragma unroll
         for (int e8 = 0; e8 < 4; ++e8) {
-          float f[8];
-          unpack8(braw[e8], IsBf16<T>::v, f);
+          const uint4 b4 = *reinterpret_cast<const uint4*>(sB + half * kBlk + sw128_off(row, h * 4 + e8));
+          const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const int i = e8 * 8 + e;
+          for (int e = 0; e < 4; ++e) {
+            const int i = e8 * 8 + 2 * e;
             const float2 t = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])),
-                                        make_float2(scale, scale), make_float2(f[e], f[e + 1]));
+                                        make_float2(scale, scale), unpack2<T>(bw[e]));
             x[i] = __float_as_uint(t.x);
             x[i + 1] = __float_as_uint(t.y);
           }
@@ -178,7 +169,6 @@ __device__ __forceinline__ float row_max(uint32_t taddr, const uint8_t* sB, int 
           if (!(bits & (1u << e))) x[e] = 0xff800000u;   // -inf
       }
       if (BIAS || CUT) tmem_st32(taddr + q * 32, x);
-      if (q < 3) load_bias(q + 1);
 #pragma unroll
       for (int e = 0; e < 32; e += 8)
 #pragma unroll

@@ -201,6 +201,13 @@ struct IsBf16 { static constexpr int v = 0; };
 template <>
 struct IsBf16<__nv_bfloat16> { static constexpr int v = 1; };
 
+// two 16-bit values of a word
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if (IsBf16<T>::v) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
