@@ -163,9 +163,26 @@ class NativeDeclined(RuntimeError):
 
 _lock = threading.Lock()
 _lib = None
+_torch_ext = None
 
-# counters the tests use to prove the native path ran
-stats = {"calls": 0, "kernel_launches": 0}
+
+class _Stats(dict):
+    """Counters the tests use to prove the native path ran: what Python counts here, plus what
+    the torch extension counts itself."""
+
+    def __getitem__(self, key):
+        n = super().__getitem__(key)
+        if _torch_ext is not None:
+            n += _torch_ext.calls() if key == "calls" else _torch_ext.launches()
+        return n
+
+    def __setitem__(self, key, value):
+        if _torch_ext is not None:
+            value -= _torch_ext.calls() if key == "calls" else _torch_ext.launches()
+        super().__setitem__(key, value)
+
+
+stats = _Stats(calls=0, kernel_launches=0)
 
 
 def load():
@@ -194,6 +211,35 @@ def load():
     return _lib
 
 
+def torch_ext():
+    """The torch side of layer norm and attention (csrc/ftm_torch.cpp), bound to the loaded
+    library's functions. `NativeLibraryMissing` when it is not built."""
+    global _torch_ext
+    if _torch_ext is not None:
+        return _torch_ext
+    lib = load()
+    with _lock:
+        if _torch_ext is not None:
+            return _torch_ext
+        import importlib.util
+        path = os.path.join(HERE, "_ftm_torch.so")
+        if not os.path.exists(path):
+            raise NativeLibraryMissing(
+                f"{path} not found: build it with `python fast_trimul_b200/csrc/build.py`")
+        try:
+            spec = importlib.util.spec_from_file_location("_ftm_torch", path)
+            ext = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(ext)
+        except ImportError as e:
+            raise NativeLibraryMissing(f"cannot load {path}: {e}") from e
+        ext.bind_library([ctypes.cast(getattr(lib, name), _vp).value for name in (
+            "ftm_layer_norm_fwd", "ftm_layer_norm_bwd", "ftm_layer_norm_bwd_workspace_bytes",
+            "ftm_attention_fwd", "ftm_attention_bwd", "ftm_attention_workspace_bytes",
+            "ftm_attention_bwd_workspace_bytes", "ftm_last_launch_count", "ftm_status_string")])
+        _torch_ext = ext
+    return _torch_ext
+
+
 def available():
     try:
         load()
@@ -214,6 +260,15 @@ def check(code, what):
     if code in (BAD_SHAPE, BAD_DTYPE, BAD_ALIGN, UNSUPPORTED_ARCH):
         raise NativeDeclined(msg)
     raise NativeKernelError(msg)
+
+
+def check_raised(error):
+    """Turn the extension's report of a failed library call into this module's errors."""
+    text = str(error)
+    if "(status " in text:
+        code = int(text.rsplit("(status ", 1)[1].split(")")[0])
+        check(code, text.split(":", 1)[0])
+    raise error
 
 
 def record_launches():

@@ -20,12 +20,10 @@ import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .norm import device_guard
 
-_DT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_TYPES = (torch.float16, torch.bfloat16)
 
 
 class AttentionErrorWord:
@@ -38,6 +36,7 @@ class AttentionErrorWord:
         self.host = torch.zeros(16, dtype=torch.int32).pin_memory()
         self.ptr, self.host_ptr = self.dev.data_ptr(), self.host.data_ptr()
         self.word = ctypes.c_int32.from_address(self.host_ptr)
+        _lib.torch_ext().set_words(self.dev.device.index, self.ptr, self.host_ptr)
 
     def poll(self):
         code = self.word.value
@@ -92,7 +91,7 @@ def _heads(q_heads, kv_heads, dim, cuda, dtype):
         raise ValueError("the head dimension is empty")
     if not cuda:
         return
-    if dtype not in _DT:
+    if dtype not in _TYPES:
         raise _lib.NativeDeclined(f"attention kernels take fp16 and bf16, got {dtype}")
     if dim % 8 or dim > 128:
         raise _lib.NativeDeclined(f"attention kernels take head dimensions that are multiples of 8 up to 128, got {dim}")
@@ -112,96 +111,21 @@ def _in_place(t):
     return t
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _native(name, *args):
+    """The extension's entry point: its result, or None where the call is not plain."""
+    try:
+        return getattr(_lib.torch_ext(), name)(*args)
+    except RuntimeError as e:
+        _lib.check_raised(e)
 
 
-class _Call:
-    """What a forward and its backward share beside the tensors: the C problem's plain fields
-    and the device arrays it points to."""
-
-    __slots__ = ("heads", "kv_heads", "dim", "causal", "scale", "seqs", "q_len", "kv_len", "cu_q", "cu_k",
-                 "lengths", "mask", "bias_seqs")
-
-    def problem(self, q, k, v, bias, out, stats):
-        """q (rows, heads, dim); k, v (rows, heads, dim) or (batch, rows, heads, dim)."""
-        b = k.dim() == 4
-        br, bh, bb = (bias.stride(2), bias.stride(1), bias.stride(0)) if bias is not None else (0, 0, 0)
-        return _lib.Attention(
-            _DT[q.dtype], self.heads, self.kv_heads, self.dim, self.causal, self.scale, self.seqs, self.q_len,
-            self.kv_len, q.shape[0], k.shape[-3], _ptr(self.cu_q), _ptr(self.cu_k), _ptr(self.lengths),
-            q.data_ptr(), q.stride(0), q.stride(1),
-            k.data_ptr(), k.stride(-3), k.stride(-2), k.stride(0) if b else 0,
-            v.data_ptr(), v.stride(-3), v.stride(-2), v.stride(0) if b else 0,
-            _ptr(self.mask), _ptr(bias), self.bias_seqs, br, bh, bb, out.data_ptr(), _ptr(stats))
-
-
-def _launch(call, q, k, v, bias, train):
-    """Forward launch; returns out, the row statistics and the packed call's tile lists (the
-    last two only when training)."""
-    lib = _lib.load()
-    dev = q.device
-    err = attention_error_word(dev)
-    err.poll()
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    stats = torch.empty(q.shape[0], call.heads, 2, dtype=torch.float32, device=dev) if train else None
-    with device_guard(q):
-        prob = call.problem(q, k, v, bias, out, stats)
-        nbytes = lib.ftm_attention_workspace_bytes(prob, train)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _lib.check(lib.ftm_attention_fwd(prob, train, _ptr(ws), nbytes, err.ptr, err.host_ptr,
-                                         torch.cuda.current_stream().cuda_stream), "ftm_attention_fwd")
-    _lib.record_launches()
-    return out, stats, ws
-
-
-class _Attention(torch.autograd.Function):
-    """Forward that keeps its output and two floats of statistics per row and head; the backward
-    recomputes the weights tile by tile. No atomics: the gradients are the same bits on every
-    call, and those of shared heads and of a shared bias are summed inside the kernels."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, bias, call):
-        q, k, v = _in_place(q), _in_place(k), _in_place(v)
-        ready = None if bias is None else _bias_in_place(bias)
-        out, stats, lists = _launch(call, q, k, v, ready, 1)
-        ctx.call = call
-        ctx.bias_shape = None if bias is None else bias.shape
-        ctx.save_for_backward(q, k, v, ready, out, stats, lists)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        q, k, v, bias, out, stats, lists = ctx.saved_tensors
-        lib = _lib.load()
-        call, dev = ctx.call, q.device
-        err = attention_error_word(dev)
-        err.poll()
-        need_q, need_k, need_v, need_b = ctx.needs_input_grad[:4]
-        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)   # noqa: E731
-        grad = _in_place(grad if grad.dtype == q.dtype else grad.to(q.dtype))
-        dq = new(q) if need_q else None
-        dk, dv = (new(k), new(v)) if need_k or need_v else (None, None)
-        db = torch.empty(ctx.bias_shape, dtype=q.dtype, device=dev) if need_b else None
-        with device_guard(q):
-            prob = call.problem(q, k, v, bias, out, stats)
-            nbytes = lib.ftm_attention_bwd_workspace_bytes(prob, 1 if need_b else 0)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            _lib.check(lib.ftm_attention_bwd(
-                prob, grad.data_ptr(), grad.stride(0), grad.stride(1), _ptr(lists),
-                0 if lists is None else lists.numel(), ws.data_ptr(), nbytes, _ptr(dq), _ptr(dk), _ptr(dv),
-                _ptr(db), err.ptr, err.host_ptr, torch.cuda.current_stream().cuda_stream), "ftm_attention_bwd")
-        _lib.record_launches()
-        return dq, dk if need_k else None, dv if need_v else None, db, None
-
-
-def _run(call, q, k, v, bias):
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
-                                    (bias is not None and bias.requires_grad)):
-        return _Attention.apply(q, k, v, bias, call)
-    return _launch(call, _in_place(q), _in_place(k), _in_place(v),
-                   None if bias is None else _bias_in_place(bias), 0)[0]
+def _prepared(name, q, *args):
+    """The same after the checks, with arguments that the kernels can read."""
+    attention_error_word(q.device).poll()
+    out = _native(name, q, *args)
+    if out is None:
+        raise _lib.NativeDeclined(f"{name} attention of {tuple(q.shape)} {q.dtype}")
+    return out
 
 
 def _as_mask(mask, device, shape, name):
@@ -269,6 +193,11 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, *, causal=True, sca
     sees keys j <= i + (keys - queries), aligned to the last key, so a prompt's continuation
     passes its new queries and all keys. scale: dim ** -0.5 if None. key_mask: (rows of k,), keys
     with 0 / False are not seen. Returns q's shape and type. Differentiable once in q, k and v."""
+    if q.is_cuda and (cu_seqlens_k is not None or q.shape[0] == k.shape[0]):
+        out = _native("packed", q, k, v, cu_seqlens, cu_seqlens if cu_seqlens_k is None else cu_seqlens_k,
+                      bool(causal), scale, key_mask)
+        if out is not None:
+            return out
     if q.dim() != 3 or k.dim() != 3 or tuple(k.shape) != tuple(v.shape) or q.shape[2] != k.shape[2]:
         raise ValueError("packed_attention needs q (rows, heads, dim) and k, v (rows, kv_heads, dim), got "
                          f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -286,11 +215,8 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, *, causal=True, sca
         return _packed_torch(q, k, v, cu_q, cu_k, causal, s, mask)
     if cu_q.numel() < 2 or q.shape[0] == 0 or k.shape[0] == 0:
         return q * 0 + (k.sum() + v.sum()) * 0 if torch.is_grad_enabled() else torch.zeros_like(q)
-    c = _Call()
-    c.heads, c.kv_heads, c.dim, c.causal, c.scale = q.shape[1], k.shape[1], q.shape[2], bool(causal), s
-    c.seqs, c.q_len, c.kv_len, c.cu_q, c.cu_k, c.lengths = cu_q.numel() - 1, 0, 0, cu_q, cu_k, None
-    c.mask, c.bias_seqs = None if mask is None else mask.contiguous(), 0
-    return _run(c, q, k, v, None)
+    return _prepared("packed", _in_place(q), _in_place(k), _in_place(v), cu_q, cu_k, bool(causal), s,
+                     None if mask is None else mask.contiguous())
 
 
 # --------------------------------------------------------------------------- cached
@@ -302,6 +228,10 @@ def cached_attention(q, k_cache, v_cache, lengths, *, scale=None):
     hold keys (read on the device, clamped to 0 .. capacity: a captured graph replays with new
     lengths). A sequence of length 0 gives zeros. Returns (B, heads, dim). For inference: there is
     no backward, and inputs that want gradients are refused."""
+    if q.is_cuda:
+        out = _native("cached", q, k_cache, v_cache, lengths, scale)
+        if out is not None:
+            return out
     if q.dim() != 3 or k_cache.dim() != 4 or tuple(k_cache.shape) != tuple(v_cache.shape) or \
             q.shape[0] != k_cache.shape[0] or q.shape[2] != k_cache.shape[3]:
         raise ValueError("cached_attention needs q (B, heads, dim) and caches (B, capacity, kv_heads, dim), got "
@@ -323,27 +253,10 @@ def cached_attention(q, k_cache, v_cache, lengths, *, scale=None):
         rows = lambda t: t.float().masked_fill(~keep[..., None, None], 0).transpose(1, 2)   # noqa: E731
         o = _attend(q.float().view(B, HK, H // HK, D), rows(k_cache), rows(v_cache), keep[:, None, None], s)
         return o.reshape(B, H, D).to(q.dtype)
-    c = _Call()
-    c.heads, c.kv_heads, c.dim, c.causal, c.scale = H, HK, D, False, s
-    c.seqs, c.q_len, c.kv_len, c.cu_q, c.cu_k, c.lengths = B, 1, 0, None, None, lens
-    c.mask, c.bias_seqs = None, 0
-    return _launch(c, _in_place(q), _in_place(k_cache), _in_place(v_cache), None, 0)[0]
+    return _prepared("cached", _in_place(q), _in_place(k_cache), _in_place(v_cache), lens, s)
 
 
 # ----------------------------------------------------------------------------- pair
-def _bias_in_place(bias):
-    """(B, heads, N, N) with rows a multiple of 8 elements apart: copied when they are not."""
-    n = bias.shape[-1]
-    if n % 8 == 0:
-        return _in_place(bias)
-    if bias.stride(-1) == 1 and bias.data_ptr() % 16 == 0 and \
-            all(s > 0 and s % 8 == 0 for s, e in zip(bias.stride()[:-1], bias.shape[:-1]) if e > 1):
-        return bias
-    wide = torch.empty(*bias.shape[:-1], (n + 7) // 8 * 8, dtype=bias.dtype, device=bias.device)
-    wide[..., :n] = bias
-    return wide[..., :n]
-
-
 def pair_attention(q, k, v, bias, mask=None, *, scale=None):
     """Attention along the rows of a pair representation, with a bias that the rows share.
 
@@ -352,6 +265,10 @@ def pair_attention(q, k, v, bias, mask=None, *, scale=None):
     False are not seen (a row that has none left gives zeros). scale: dim ** -0.5 if None. Returns
     q's shape and type. Triangle attention has R = N; R = 1 is attention of a single representation
     with pair bias. Differentiable once in q, k, v and bias (its gradient summed over the rows)."""
+    if q.is_cuda:
+        out = _native("pair", q, k, v, bias, mask, scale)
+        if out is not None:
+            return out
     if q.dim() != 5 or tuple(k.shape) != tuple(q.shape) or tuple(v.shape) != tuple(q.shape):
         raise ValueError("pair_attention needs q, k and v of one shape (B, R, N, heads, dim), got "
                          f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -370,10 +287,4 @@ def pair_attention(q, k, v, bias, mask=None, *, scale=None):
         o = _attend(q.float().transpose(2, 3), rows(k), rows(v), keep[:, :, None, None, :], s,
                     None if bias is None else bias.float()[:, None])
         return o.transpose(2, 3).to(q.dtype)
-    c = _Call()
-    c.heads, c.kv_heads, c.dim, c.causal, c.scale = H, H, D, False, s
-    c.seqs, c.q_len, c.kv_len, c.cu_q, c.cu_k, c.lengths = B * R, N, N, None, None, None
-    c.mask = None if m is None else m.contiguous()
-    c.bias_seqs = 0 if bias is None else B * R // bias.shape[0]
-    flat = lambda t: t.reshape(B * R * N, H, D)   # noqa: E731
-    return _run(c, flat(q), flat(k), flat(v), bias).view(B, R, N, H, D)
+    return _prepared("pair", _in_place(q), _in_place(k), _in_place(v), bias, None if m is None else m.contiguous(), s)

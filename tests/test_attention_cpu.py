@@ -172,3 +172,17 @@ def test_fused_trunk_equals_the_plain_one(masked):
     assert torch.allclose(z1[:, :n, :n], z2[:, :n, :n], atol=1e-4)
     if not masked:      # the single attention has no mask: padded rows of z reach it
         assert torch.allclose(s1, s2, atol=1e-4)
+
+
+def test_torch_extension_loads_and_leaves_cpu_calls_alone():
+    ext = _lib.torch_ext()
+    x = torch.randn(3, 8)
+    assert ext.layer_norm(x, None, None, 1e-5) is None
+    q = torch.randn(4, 2, 8)
+    cu = ends([4])
+    assert ext.packed(q, q, q, cu, cu, True, None, None) is None
+    assert ext.cached(q, q[:, None], q[:, None], torch.ones(4, dtype=torch.int32), None) is None
+    assert ext.pair(q[None, None], q[None, None], q[None, None], None, None, None) is None
+    n = _lib.stats["calls"]
+    _lib.stats["calls"] += 2
+    assert _lib.stats["calls"] == n + 2
