@@ -139,8 +139,9 @@ BwdSpace bwd_space(const ftm_attention* p, int want_dbias, int sms) {
     const int64_t biases = p->sequences / p->bias_seqs;
     const int64_t tiles = biases * p->heads * ((p->q_len + kTileRows - 1) / kTileRows) *
                           ((p->kv_len + kTileRows - 1) / kTileRows);
-    int64_t splits = (sms + tiles - 1) / tiles;
+    int64_t splits = sms / tiles;      // one item per SM at most: a second wave would be mostly idle
     if (splits > p->bias_seqs) splits = p->bias_seqs;
+    if (splits < 1) splits = 1;
     w.splits = static_cast<int>(splits);
     if (splits > 1)
       w.total += up256(size_t(splits) * biases * p->heads * p->q_len * p->kv_len * sizeof(float));

@@ -18,6 +18,8 @@
 // TMA (and, in dkv, the per-query constants), warp 9 MMA. All 512 TMEM columns, one block
 // per SM: dq holds S twice (the next tile's scores are formed under this one's
 // elementwise part), dkv holds S^T, dP^T, dV, dK.
+#include <climits>
+
 #include "ftm_attention.cuh"
 
 namespace ftm {
@@ -26,7 +28,7 @@ namespace {
 enum : int { KERNEL_DQ = 5, KERNEL_DKV = 6, KERNEL_DBIAS = 7 };
 constexpr int kBwdThreads = 320;
 
-// bstats of a (row, head): without a bias x = m c + log2(l) with c = scale log2(e), so that
+// bstats[head][row], so that a tile's are read in whole lines: without a bias x = m c + log2(l) with c = scale log2(e), so that
 // p = 2^(c s - x); with one x = m, y = log2(l), p = 2^((t - x) log2(e) - y), which stays
 // exact for scores near the type's lowest value. z = rowsum(g * o). A row without keys has
 // log2(l) = inf, hence p = 0.
@@ -54,7 +56,7 @@ attn_delta_kernel(const __grid_constant__ AttnArgs a, int lanes, int bias) {
     for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (i < n && l == 0) {
       const float2 st = a.stats[i];
-      a.bstats[i] = bias ? make_float4(st.x, st.y, s, 0.f) : make_float4(fmaf(st.x, c, st.y), 0.f, s, 0.f);
+      a.bstats[static_cast<size_t>(i % a.heads) * a.q_rows + i / a.heads] = bias ? make_float4(st.x, st.y, s, 0.f) : make_float4(fmaf(st.x, c, st.y), 0.f, s, 0.f);
     }
   }
   grid_dep_release();
@@ -287,7 +289,8 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       const bool live = tok < it.nq && row < a.group * a.tq;
       const size_t orow = (static_cast<size_t>(it.q0) + tok) * a.heads + it.head * a.group + gi;
       const int seen = a.causal ? min(it.klen, it.pos0 + tok + it.off + 1) : it.klen;
-      const float4 st = live ? a.bstats[orow] : make_float4(0.f, INFINITY, 0.f, 0.f);
+      const float4 st = live ? a.bstats[static_cast<size_t>(it.head * a.group + gi) * a.q_rows + it.q0 + tok]
+                             : make_float4(0.f, INFINITY, 0.f, 0.f);
       const float ref = BIAS || live ? st.x : INFINITY;
       for (int kt = it.kt0; kt < it.kt1; ++kt, ++kn) {
         const int b = kn & 1;
@@ -462,6 +465,14 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     const uint32_t q_bytes = DP / 64 * 128u * (a.group * a.tq);
     int in = 0, qn = 0;
     bool ok = true;
+    int col_tok[4];          // token of this lane's columns (past all tiles: none), and the place of
+    size_t col_off[4];       // its constants behind the tile's first
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int r = w * 32 + lane, tok = r / a.group;
+      col_tok[w] = r < a.group * a.tq ? tok : INT_MAX;
+      col_off[w] = static_cast<size_t>(r - tok * a.group) * a.q_rows + tok;
+    }
     for (; ok && walk_item<true>(a, n, it); n += gridDim.x) {
       if (it.kt1 <= it.kt0) continue;
       ok = mbar_wait_warp(kv_empty, (in & 1) ^ 1, a.err, err_code(KERNEL_DKV, ROLE_PRODUCER, 1));
@@ -494,20 +505,26 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         }
         ++qn;
         __syncwarp();
-        // the constants of this tile's queries, one per column of S^T
+        // the constants of this tile's queries, one per column of S^T: four loads in flight
+        // (behind conditions they came one after the other, 4900 clocks a tile)
+        float4 st[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int left = it.nq - t * a.tq;
+          const bool live = col_tok[w] < left;
+          const size_t at = live ? static_cast<size_t>(it.head) * a.group * a.q_rows + it.q0 + t * a.tq + col_off[w] : 0;
+          st[w] = a.bstats[at];
+          if (!live) st[w] = make_float4(BIAS ? 0.f : INFINITY, INFINITY, 0.f, 0.f);   // p = 0
+        }
         const int cn = qn - 1, cb = cn % C::kCols;
         ok = mbar_wait_warp(&c_empty[cb], ((cn / C::kCols) & 1) ^ 1, a.err, err_code(KERNEL_DKV, ROLE_PRODUCER, 5));
         if (!ok) break;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const int r = w * 32 + lane, tok = r / a.group;
-          const bool live = r < a.group * a.tq && t * a.tq + tok < it.nq;
-          float4 st = make_float4(BIAS ? 0.f : INFINITY, INFINITY, 0.f, 0.f);   // p = 0
-          if (live)
-            st = a.bstats[(static_cast<size_t>(it.q0) + t * a.tq + tok) * a.heads + it.head * a.group + r - tok * a.group];
-          sC[cb * 384 + r] = st.x;
-          sC[cb * 384 + 128 + r] = st.y;
-          sC[cb * 384 + 256 + r] = st.z;
+          const int r = w * 32 + lane;
+          sC[cb * 384 + r] = st[w].x;
+          sC[cb * 384 + 128 + r] = st[w].y;
+          sC[cb * 384 + 256 + r] = st[w].z;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&c_full[cb]);
@@ -871,7 +888,7 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
         it.k0 = seq * a.k_len;
         uint32_t keep[4];
         key_bits(a, it, kt, lane, keep);
-        const float4 st = live ? a.bstats[(static_cast<size_t>(seq) * a.q_len + pos) * a.heads + head]
+        const float4 st = live ? a.bstats[static_cast<size_t>(head) * a.q_rows + static_cast<size_t>(seq) * a.q_len + pos]
                                : make_float4(0.f, INFINITY, 0.f, 0.f);
         ok = mbar_wait_warp(&t_full[tb], (rn >> 1) & 1, a.err, err_code(KERNEL_DBIAS, ROLE_EPILOGUE, 2));
         if (!ok) break;
