@@ -147,21 +147,8 @@ __device__ __forceinline__ float row_max(uint32_t taddr, const uint8_t* sB, int 
       uint32_t(&x)[32] = r[h];
       tmem_wait_ld();
       if (q < 3) FTM_TMEM_LD32_NOWAIT(taddr + (q + 1) * 32, r[h ^ 1]);
-      if (BIAS) {   // scores with the bias go back over the plain ones
-#pragma unroll
-        for (int e8 = 0; e8 < 4; ++e8) {
-          const uint4 b4 = *reinterpret_cast<const uint4*>(sB + half * kBlk + sw128_off(row, h * 4 + e8));
-          const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = e8 * 8 + 2 * e;
-            const float2 t = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])),
-                                        make_float2(scale, scale), unpack2<T>(bw[e]));
-            x[i] = __float_as_uint(t.x);
-            x[i + 1] = __float_as_uint(t.y);
-          }
-        }
-      }
+      // scores with the bias go back over the plain ones
+      if (BIAS) add_bias<T>(x, sB + half * kBlk, row, h * 4, scale);
       if (CUT) {
         const uint32_t bits = (half ? keep[2 + h] : keep[h]) & bits_below(lim, q);
 #pragma unroll

@@ -309,6 +309,24 @@ __device__ __forceinline__ void key_bits(const AttnArgs& a, const Item& it, int 
   }
 }
 
+// r = scale r + bias for 32 columns: chunks `chunk0` to chunk0 + 3 of row `row` of a bias block
+template <typename T>
+__device__ __forceinline__ void add_bias(uint32_t (&r)[32], const uint8_t* block, int row, int chunk0, float scale) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint4 b4 = *reinterpret_cast<const uint4*>(block + sw128_off(row, chunk0 + q));
+    const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = q * 8 + 2 * e;
+      const float2 t = __ffma2_rn(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])),
+                                  make_float2(scale, scale), unpack2<T>(bw[e]));
+      r[i] = __float_as_uint(t.x);
+      r[i + 1] = __float_as_uint(t.y);
+    }
+  }
+}
+
 // bits [0, lim) of a 128-bit row
 __device__ __forceinline__ uint32_t bits_below(int lim, int word) {
   const int n = lim - word * 32;

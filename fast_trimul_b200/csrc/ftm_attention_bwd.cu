@@ -14,9 +14,10 @@
 // time, at the price of forming S and dP twice (7 products instead of 5). fp32 everywhere
 // but the 16-bit operands P and dS, rounded once like the inputs of any product here.
 //
-// Roles: warps 0-7 elementwise (two per TMEM lane quarter, each half of the columns), warp 8
-// TMA (and, in dkv, the per-query constants), warp 9 MMA. All 512 TMEM columns, one block
-// per SM: dq holds S twice (the next tile's scores are formed under this one's
+// Roles: warps 0-15 elementwise (four per TMEM lane quarter, 32 of the columns each), warp 16
+// TMA (and, in dkv, the per-query constants), warp 17 MMA. The elementwise part is the long
+// one, and bound by latency: with 8 warps it took 3450 clocks of a dkv tile's 3800 at dim 128
+// (the products take 2048). All 512 TMEM columns, one block per SM: dq holds S twice (the next tile's scores are formed under this one's
 // elementwise part), dkv holds S^T, dP^T, dV, dK.
 #include <climits>
 
@@ -26,7 +27,8 @@ namespace ftm {
 namespace {
 
 enum : int { KERNEL_DQ = 5, KERNEL_DKV = 6, KERNEL_DBIAS = 7 };
-constexpr int kBwdThreads = 320;
+constexpr int kBwdThreads = 576;
+constexpr int kTmaWarp = 16, kMmaWarp = 17, kElemWarps = 16;
 
 // bstats[head][row], so that a tile's are read in whole lines: without a bias x = m c + log2(l) with c = scale log2(e), so that
 // p = 2^(c s - x); with one x = m, y = log2(l), p = 2^((t - x) log2(e) - y), which stays
@@ -77,19 +79,19 @@ __device__ __forceinline__ void zero_outside(const int* cu, int seqs, int rows, 
 template <int COLS, typename T>
 __device__ __forceinline__ void store_acc(uint32_t taddr, int col0, int dim, float f, bool live, bool any, T* out) {
 #pragma unroll
-  for (int q = 0; q < COLS / 32; ++q) {
-    uint32_t o[32];
+  for (int q = 0; q < COLS / 16; ++q) {
+    uint32_t o[16];
     if (any) {
-      FTM_TMEM_LD32_NOWAIT(taddr + col0 + q * 32, o);
+      tmem_ld16_nowait(taddr + col0 + q * 16, o);
       tmem_wait_ld();
     } else {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] = 0;
+      for (int e = 0; e < 16; ++e) o[e] = 0;
     }
     if (!live) continue;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int c = col0 + q * 32 + e * 8;
+    for (int e = 0; e < 2; ++e) {
+      const int c = col0 + q * 16 + e * 8;
       if (c >= dim) break;
       float x[8];
 #pragma unroll
@@ -98,6 +100,14 @@ __device__ __forceinline__ void store_acc(uint32_t taddr, int col0, int dim, flo
           make_uint4(pack16<T>(x[0], x[1]), pack16<T>(x[2], x[3]), pack16<T>(x[4], x[5]), pack16<T>(x[6], x[7]));
     }
   }
+}
+
+// the bits of key_bits() for this warp's 32 columns of tile kt
+__device__ __forceinline__ uint32_t key_word(const AttnArgs& a, const Item& it, int kt, int part, int lane) {
+  const int c = kt * kTileRows + part * 32 + lane;
+  bool on = c < it.klen;
+  if (on && a.key_mask) on = a.key_mask[static_cast<size_t>(it.k0) + c] != 0;
+  return __ballot_sync(0xffffffffu, on);
 }
 
 // --------------------------------------------------------------------------------- dq
@@ -142,10 +152,10 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
 
   const int warp = uniform<E>(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 18; ++i) mbar_init(q_full + i, i == 11 || i == 15 ? 8 : 1);
+    for (int i = 0; i < 18; ++i) mbar_init(q_full + i, i == 11 || i == 15 ? kElemWarps : 1);
     fence_mbar_init();
   }
-  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -156,7 +166,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
   int n = blockIdx.x;
   Item it;
 
-  if (warp == 8) {
+  if (warp == kTmaWarp) {
     const uint32_t q_bytes = 2u * (DP / 64 * 128u * (a.group * a.tq));
     int qn = 0, kn = 0;
     bool ok = true;
@@ -200,7 +210,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       }
       if (BIAS && kn) mbar_wait_drain(b_full, (kn - 1) & 1);
     }
-  } else if (warp == 9) {
+  } else if (warp == kMmaWarp) {
     constexpr uint32_t id_s = idesc_f16(IsBf16<T>::v, 128, 128, 0, 0);
     constexpr uint32_t id_o = idesc_f16(IsBf16<T>::v, 128, DP, 0, 1);
     const uint32_t q_addr = smem_u32(sQ), g_addr = smem_u32(sG);
@@ -275,14 +285,14 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       mbar_wait_drain(drain, 0);
     }
   } else {
-    const int quad = warp & 3, half = warp >> 2;
+    const int quad = warp & 3, part = warp >> 2;   // columns 32 part and on
     const int row = quad * 32 + lane;
     const int tok = row / a.group, gi = row - tok * a.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float c = log2_scale(a.scale);
     T* dq = static_cast<T*>(a.dq);
     if (a.walk == WALK_LIST)
-      zero_outside(a.cu_q, a.seqs, a.q_rows, static_cast<long long>(a.heads) * a.dim / 8, dq, threadIdx.x, 256);
+      zero_outside(a.cu_q, a.seqs, a.q_rows, static_cast<long long>(a.heads) * a.dim / 8, dq, threadIdx.x, kElemWarps * 32);
     int kn = 0, qn = 0;
     bool ok = true;
     for (; ok && walk_item<false>(a, n, it); n += gridDim.x) {
@@ -294,77 +304,50 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       const float ref = BIAS || live ? st.x : INFINITY;
       for (int kt = it.kt0; kt < it.kt1; ++kt, ++kn) {
         const int b = kn & 1;
-        const int lim = seen - kt * kTileRows;
-        uint32_t keep[4];
-        bool cut = lim < kTileRows;
-        if (a.key_mask) {
-          key_bits(a, it, kt, lane, keep);
-          cut = cut || (keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu;
-        } else {
-          keep[0] = keep[1] = keep[2] = keep[3] = 0xffffffffu;
-        }
-        cut = __any_sync(0xffffffffu, cut);
+        const uint32_t on = (a.key_mask ? key_word(a, it, kt, part, lane) : 0xffffffffu) &
+                            bits_below(seen - kt * kTileRows, part);
+        const bool cut = __any_sync(0xffffffffu, on != 0xffffffffu);
         ok = mbar_wait_warp(&s_full[b], (kn >> 1) & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 1));
         if (BIAS) ok = ok && mbar_wait_warp(b_full, kn & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 2));
         if (!ok) break;
         tc_fence_after();
         const uint32_t scol = lanes + (b ? 384 : 0);
-        uint32_t r[2][32];
-        FTM_TMEM_LD32_NOWAIT(scol + half * 64, r[0]);
-        FTM_TMEM_LD32_NOWAIT(scol + half * 64 + 32, r[1]);
+        uint32_t r[32];
+        FTM_TMEM_LD32_NOWAIT(scol + part * 32, r);
         tmem_wait_ld();
         if (BIAS) {
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            float f[8];
-            unpack8(*reinterpret_cast<const uint4*>(sB + half * kBlk + sw128_off(row, q)), IsBf16<T>::v, f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              uint32_t& x = r[q >> 2][(q & 3) * 8 + e];
-              x = __float_as_uint(fmaf(__uint_as_float(x), a.scale, f[e]));
-            }
-          }
+          add_bias<T>(r, sB + (part >> 1) * kBlk, row, (part & 1) * 4, a.scale);
           __syncwarp();
           if (lane == 0) mbar_arrive(b_empty);
         }
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float x = __uint_as_float(r[q][e]);
-            r[q][e] = __float_as_uint(ex2(BIAS ? fmaf(x - ref, kLog2e, -st.y) : fmaf(x, c, -ref)));
-          }
+        for (int e = 0; e < 32; ++e) {
+          const float x = __uint_as_float(r[e]);
+          r[e] = __float_as_uint(ex2(BIAS ? fmaf(x - ref, kLog2e, -st.y) : fmaf(x, c, -ref)));
+        }
         if (cut) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const uint32_t on = keep[half * 2 + q] & bits_below(lim, half * 2 + q);
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((on >> e) & 1u)) r[q][e] = 0u;
-          }
+          for (int e = 0; e < 32; ++e)
+            if (!(on & (1u << e))) r[e] = 0u;
         }
         ok = mbar_wait_warp(dp_full, kn & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 3));
         if (!ok) break;
         tc_fence_after();
-        uint32_t pk[32];
+        uint32_t pk[16], d[32];
+        FTM_TMEM_LD32_NOWAIT(lanes + 128 + part * 32, d);
+        tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t d[32];
-          FTM_TMEM_LD32_NOWAIT(lanes + 128 + half * 64 + q * 32, d);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float x0 = __uint_as_float(r[q][e]) * (__uint_as_float(d[e]) - st.z);
-            float x1 = __uint_as_float(r[q][e + 1]) * (__uint_as_float(d[e + 1]) - st.z);
-            if (cut) {   // a key that is not seen gives nothing, whatever its V holds
-              x0 = r[q][e] ? x0 : 0.f;
-              x1 = r[q][e + 1] ? x1 : 0.f;
-            }
-            pk[q * 16 + e / 2] = pack16<T>(x0, x1);
+        for (int e = 0; e < 32; e += 2) {
+          float x0 = __uint_as_float(r[e]) * (__uint_as_float(d[e]) - st.z);
+          float x1 = __uint_as_float(r[e + 1]) * (__uint_as_float(d[e + 1]) - st.z);
+          if (cut) {   // a key that is not seen gives nothing, whatever its V holds
+            x0 = r[e] ? x0 : 0.f;
+            x1 = r[e + 1] ? x1 : 0.f;
           }
+          pk[e / 2] = pack16<T>(x0, x1);
         }
-        named_barrier_sync(1 + quad, 64);   // both halves have read S: dS goes over it
-        tmem_st32(scol + half * 32, pk);
+        named_barrier_sync(1 + quad, 128);   // the whole row of S has been read: dS goes over it
+        tmem_st16(scol + part * 16, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -378,7 +361,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
         ++qn;
         tc_fence_after();
       }
-      store_acc<DP / 2>(lanes + 256, half * (DP / 2), a.dim, a.scale, live, any, dq + orow * a.dim);
+      store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, a.scale, live, any, dq + orow * a.dim);
       tc_fence_before();
     }
   }
@@ -386,7 +369,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
   __syncthreads();
   tc_fence_after();
   __syncwarp();
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
 // -------------------------------------------------------------------------------- dkv
@@ -438,7 +421,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   const int warp = uniform<E>(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 22; ++i)
-      mbar_init(kv_full + i, i == 11 || i == 14 || i == 15 || i == 17 || i == 19 ? 8 : 1);
+      mbar_init(kv_full + i, i == 11 || i == 14 || i == 15 || i == 17 || i == 19 ? kElemWarps : 1);
     fence_mbar_init();
   }
   // rows of a query tile that no load writes (128 is no multiple of the group): zero once
@@ -450,7 +433,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       fence_proxy_async_smem();
     }
   }
-  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -461,7 +444,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   int n = blockIdx.x;
   Item it;
 
-  if (warp == 8) {
+  if (warp == kTmaWarp) {
     const uint32_t q_bytes = DP / 64 * 128u * (a.group * a.tq);
     int in = 0, qn = 0;
     bool ok = true;
@@ -538,7 +521,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       }
       if (BIAS && qn) mbar_wait_drain(b_full, (qn - 1) & 1);
     }
-  } else if (warp == 9) {
+  } else if (warp == kMmaWarp) {
     constexpr uint32_t id_s = idesc_f16(IsBf16<T>::v, 128, 128, 0, 0);
     constexpr uint32_t id_o = idesc_f16(IsBf16<T>::v, 128, DP, 0, 1);
     const uint32_t k_addr = smem_u32(sK), v_addr = smem_u32(sV);
@@ -617,15 +600,15 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       mbar_wait_drain(drain, 0);
     }
   } else {
-    const int quad = warp & 3, half = warp >> 2;
+    const int quad = warp & 3, part = warp >> 2;   // columns 32 part and on
     const int row = quad * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float c = log2_scale(a.scale);
     T *dk = static_cast<T*>(a.dk), *dv = static_cast<T*>(a.dv);
     if (a.walk == WALK_LIST) {
       const long long per = static_cast<long long>(a.kv_heads) * a.dim / 8;
-      zero_outside(a.cu_k, a.seqs, a.kv_rows, per, dk, threadIdx.x, 256);
-      zero_outside(a.cu_k, a.seqs, a.kv_rows, per, dv, threadIdx.x, 256);
+      zero_outside(a.cu_k, a.seqs, a.kv_rows, per, dk, threadIdx.x, kElemWarps * 32);
+      zero_outside(a.cu_k, a.seqs, a.kv_rows, per, dv, threadIdx.x, kElemWarps * 32);
     }
     int qn = 0, in = 0;
     bool ok = true;
@@ -647,59 +630,46 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         ok = ok && mbar_wait_warp(s_full, qn & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 3));
         if (!ok) break;
         tc_fence_after();
-        uint32_t r[2][32];
-        FTM_TMEM_LD32_NOWAIT(lanes + half * 64, r[0]);
-        FTM_TMEM_LD32_NOWAIT(lanes + half * 64 + 32, r[1]);
+        uint32_t r[32];
+        FTM_TMEM_LD32_NOWAIT(lanes + part * 32, r);
         tmem_wait_ld();
         if (BIAS) {
           // the bias of (query, this key): rows of the tile are queries
           const uint8_t* bt = sB + (row >> 6) * kBlk + (row & 7) * 2;
 #pragma unroll
-          for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int cq = half * 64 + q * 32 + e;
-              const T bv = *reinterpret_cast<const T*>(bt + sw128_off(cq, (row & 63) >> 3));
-              r[q][e] = __float_as_uint(fmaf(__uint_as_float(r[q][e]), a.scale, static_cast<float>(bv)));
-            }
+          for (int e = 0; e < 32; ++e) {
+            const T bv = *reinterpret_cast<const T*>(bt + sw128_off(part * 32 + e, (row & 63) >> 3));
+            r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), a.scale, static_cast<float>(bv)));
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(b_empty);
         }
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const int cq = half * 64 + q * 32 + e;
-            const float4 x4 = *reinterpret_cast<const float4*>(col + cq);
-            const float xs[4] = {x4.x, x4.y, x4.z, x4.w};
-            float ys[4] = {0.f, 0.f, 0.f, 0.f};
-            if (BIAS) {
-              const float4 y4 = *reinterpret_cast<const float4*>(col + 128 + cq);
-              ys[0] = y4.x; ys[1] = y4.y; ys[2] = y4.z; ys[3] = y4.w;
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float x = __uint_as_float(r[q][e + k]);
-              r[q][e + k] = __float_as_uint(ex2(BIAS ? fmaf(x - xs[k], kLog2e, -ys[k]) : fmaf(x, c, -xs[k])));
-            }
+        for (int e = 0; e < 32; e += 4) {
+          const float4 x4 = *reinterpret_cast<const float4*>(col + part * 32 + e);
+          const float xs[4] = {x4.x, x4.y, x4.z, x4.w};
+          float ys[4] = {0.f, 0.f, 0.f, 0.f};
+          if (BIAS) {
+            const float4 y4 = *reinterpret_cast<const float4*>(col + 128 + part * 32 + e);
+            ys[0] = y4.x; ys[1] = y4.y; ys[2] = y4.z; ys[3] = y4.w;
           }
-        if (cut) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const uint32_t bits = on ? ~bits_below(lo, half * 2 + q) : 0u;
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((bits >> e) & 1u)) r[q][e] = 0u;
+          for (int k = 0; k < 4; ++k) {
+            const float x = __uint_as_float(r[e + k]);
+            r[e + k] = __float_as_uint(ex2(BIAS ? fmaf(x - xs[k], kLog2e, -ys[k]) : fmaf(x, c, -xs[k])));
           }
         }
-        uint32_t pk[32];
+        if (cut) {
+          const uint32_t bits = on ? ~bits_below(lo, part) : 0u;
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+          for (int e = 0; e < 32; ++e)
+            if (!(bits & (1u << e))) r[e] = 0u;
+        }
+        uint32_t pk[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            pk[q * 16 + e / 2] = pack16<T>(__uint_as_float(r[q][e]), __uint_as_float(r[q][e + 1]));
-        named_barrier_sync(1 + quad, 64);   // both halves have read S^T: P^T goes over it
-        tmem_st32(lanes + half * 32, pk);
+        for (int e = 0; e < 32; e += 2) pk[e / 2] = pack16<T>(__uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+        named_barrier_sync(1 + quad, 128);   // the whole row of S^T has been read: P^T goes over it
+        tmem_st16(lanes + part * 16, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -707,29 +677,26 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         ok = mbar_wait_warp(dp_full, qn & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 4));
         if (!ok) break;
         tc_fence_after();
+        uint32_t d[32];
+        FTM_TMEM_LD32_NOWAIT(lanes + 128 + part * 32, d);
+        tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t d[32];
-          FTM_TMEM_LD32_NOWAIT(lanes + 128 + half * 64 + q * 32, d);
-          tmem_wait_ld();
+        for (int e = 0; e < 32; e += 4) {
+          const float4 z = *reinterpret_cast<const float4*>(col + 256 + part * 32 + e);
+          const float zs[4] = {z.x, z.y, z.z, z.w};
+          float x[4];
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 z = *reinterpret_cast<const float4*>(col + 256 + half * 64 + q * 32 + e);
-            const float zs[4] = {z.x, z.y, z.z, z.w};
-            float x[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              x[k] = __uint_as_float(r[q][e + k]) * (__uint_as_float(d[e + k]) - zs[k]);
-              if (cut) x[k] = r[q][e + k] ? x[k] : 0.f;
-            }
-            pk[q * 16 + e / 2] = pack16<T>(x[0], x[1]);
-            pk[q * 16 + e / 2 + 1] = pack16<T>(x[2], x[3]);
+          for (int k = 0; k < 4; ++k) {
+            x[k] = __uint_as_float(r[e + k]) * (__uint_as_float(d[e + k]) - zs[k]);
+            if (cut) x[k] = r[e + k] ? x[k] : 0.f;
           }
+          pk[e / 2] = pack16<T>(x[0], x[1]);
+          pk[e / 2 + 1] = pack16<T>(x[2], x[3]);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&c_empty[cb]);
-        named_barrier_sync(1 + quad, 64);
-        tmem_st32(lanes + 128 + half * 32, pk);
+        named_barrier_sync(1 + quad, 128);
+        tmem_st16(lanes + 128 + part * 16, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -743,8 +710,8 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         ++in;
         tc_fence_after();
       }
-      store_acc<DP / 2>(lanes + 256, half * (DP / 2), a.dim, 1.f, live, any, dv + orow * a.dim);
-      store_acc<DP / 2>(lanes + 384, half * (DP / 2), a.dim, a.scale, live, any, dk + orow * a.dim);
+      store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, 1.f, live, any, dv + orow * a.dim);
+      store_acc<DP / 4>(lanes + 384, part * (DP / 4), a.dim, a.scale, live, any, dk + orow * a.dim);
       tc_fence_before();
     }
   }
@@ -752,7 +719,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   __syncthreads();
   tc_fence_after();
   __syncwarp();
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
 // ------------------------------------------------------------------------------ dbias
@@ -785,10 +752,10 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + 11);
   const int warp = uniform<E>(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 11; ++i) mbar_init(full + i, i == 6 || i == 7 || i == 9 ? 8 : 1);
+    for (int i = 0; i < 11; ++i) mbar_init(full + i, i == 6 || i == 7 || i == 9 ? kElemWarps : 1);
     fence_mbar_init();
   }
-  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -812,7 +779,7 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
     r1 = static_cast<int>(static_cast<long long>(a.bias_seqs) * (split + 1) / a.splits);
   };
 
-  if (warp == 8) {
+  if (warp == kTmaWarp) {
     if (lane == 0) {
       int rn = 0, in = 0;
       bool ok = true;
@@ -841,7 +808,7 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
       for (int i = rn > NS ? rn - NS : 0; i < rn; ++i) mbar_wait_drain(&full[i % NS], (i / NS) & 1);
       if (in) mbar_wait_drain(b_full, (in - 1) & 1);
     }
-  } else if (warp == 9) {
+  } else if (warp == kMmaWarp) {
     if (lane == 0) {
       constexpr uint32_t id_s = idesc_f16(IsBf16<T>::v, 128, 128, 0, 0);
       int rn = 0;
@@ -866,7 +833,7 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
       mbar_wait_drain(drain, 0);
     }
   } else {
-    const int quad = warp & 3, half = warp >> 2;
+    const int quad = warp & 3, part = warp >> 2;   // columns 32 part and on
     const int row = quad * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     int rn = 0, in = 0;
@@ -880,14 +847,13 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
       ok = mbar_wait_warp(b_full, in & 1, a.err, err_code(KERNEL_DBIAS, ROLE_EPILOGUE, 1));
       if (!ok) break;
       ++in;
-      float acc[64];
+      float acc[32];
 #pragma unroll
-      for (int e = 0; e < 64; ++e) acc[e] = 0.f;
+      for (int e = 0; e < 32; ++e) acc[e] = 0.f;
       for (int r = r0; r < r1; ++r, ++rn) {
         const int tb = rn & 1, seq = bb * a.bias_seqs + r;
         it.k0 = seq * a.k_len;
-        uint32_t keep[4];
-        key_bits(a, it, kt, lane, keep);
+        const uint32_t on = key_word(a, it, kt, part, lane);
         const float4 st = live ? a.bstats[static_cast<size_t>(head) * a.q_rows + static_cast<size_t>(seq) * a.q_len + pos]
                                : make_float4(0.f, INFINITY, 0.f, 0.f);
         ok = mbar_wait_warp(&t_full[tb], (rn >> 1) & 1, a.err, err_code(KERNEL_DBIAS, ROLE_EPILOGUE, 2));
@@ -895,22 +861,23 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
         tc_fence_after();
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          uint32_t x[32], d[32];
-          FTM_TMEM_LD32_NOWAIT(lanes + tb * 256 + half * 64 + q * 32, x);
-          FTM_TMEM_LD32_NOWAIT(lanes + tb * 256 + 128 + half * 64 + q * 32, d);
+          uint32_t x[16], d[16];
+          tmem_ld16_nowait(lanes + tb * 256 + part * 32 + q * 16, x);
+          tmem_ld16_nowait(lanes + tb * 256 + 128 + part * 32 + q * 16, d);
           tmem_wait_ld();
-          const uint32_t on = keep[half * 2 + q];
 #pragma unroll
-          for (int e8 = 0; e8 < 4; ++e8) {
-            float f[8];
-            unpack8(*reinterpret_cast<const uint4*>(sB + half * kBlk + sw128_off(row, q * 4 + e8)), IsBf16<T>::v, f);
+          for (int e8 = 0; e8 < 2; ++e8) {
+            const uint4 b4 = *reinterpret_cast<const uint4*>(sB + (part >> 1) * kBlk +
+                                                             sw128_off(row, (part & 1) * 4 + q * 2 + e8));
+            const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const int k = e8 * 8 + e;
-              const float t = fmaf(__uint_as_float(x[k]), a.scale, f[e]);
+              const float2 f = unpack2<T>(bw[e >> 1]);
+              const float t = fmaf(__uint_as_float(x[k]), a.scale, e & 1 ? f.y : f.x);
               const float p = ex2(fmaf(t - st.x, kLog2e, -st.y));
               const float ds = p * (__uint_as_float(d[k]) - st.z);
-              acc[q * 32 + k] += (on >> k) & 1u ? ds : 0.f;
+              acc[q * 16 + k] += on & (1u << (q * 16 + k)) ? ds : 0.f;
             }
           }
         }
@@ -925,8 +892,8 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
         const size_t at = ((static_cast<size_t>(bb) * a.heads + head) * a.q_len + pos) * a.k_len;
         const size_t all = static_cast<size_t>(biases) * a.heads * a.q_len * a.k_len;
 #pragma unroll
-        for (int e = 0; e < 64; ++e) {
-          const int col = kt * kTileRows + half * 64 + e;
+        for (int e = 0; e < 32; ++e) {
+          const int col = kt * kTileRows + part * 32 + e;
           if (col >= a.k_len) break;
           if (a.splits == 1) static_cast<T*>(a.dbias)[at + col] = T(acc[e]);
           else a.dbias_part[split * all + at + col] = acc[e];
@@ -938,7 +905,7 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
   __syncthreads();
   tc_fence_after();
   __syncwarp();
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
 // dbias = sum of the splits' parts, in order
