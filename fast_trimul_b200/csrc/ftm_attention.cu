@@ -351,7 +351,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     // ------------------------------------------------------------------------ MMA
     constexpr uint32_t id_s = idesc_f16(IsBf16<T>::v, 128, 128, 0, 0);
     constexpr uint32_t id_o = idesc_f16(IsBf16<T>::v, 128, DP, 0, 1);
-    const uint32_t q_addr = smem_u32(sQ);
+    const uint32_t q_addr = uniform<E>(smem_u32(sQ));
     int qn = 0, kn = 0;        // items with keys; key tiles
     bool ok = true;
     Item next;                 // found while this item's tiles are at work
@@ -368,13 +368,14 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         return mbar_wait_warp(&k_full[kj % NS], (kj / NS) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 4));
       };
       auto scores = [&](int j) {
-        const int s = (kn + j) % NS;
+        const uint32_t s = uniform<E>((kn + j) % NS);
+        const uint32_t k_addr = uniform<E>(smem_u32(sK + s * C::kTile)), last = uniform<E>(j == n - 1);
         tc_fence_after();
         if (issuer<E>(lane)) {
-          mma_rows<E>(tmem, q_addr, smem_u32(sK + s * C::kTile), id_s, a.ksteps);
+          mma_rows<E>(tmem, q_addr, k_addr, id_s, a.ksteps);
           umma_commit(s_full);
           umma_commit(&k_empty[s]);
-          if (j == n - 1) umma_commit(q_empty);
+          if (last) umma_commit(q_empty);
         }
         __syncwarp();
       };
@@ -411,11 +412,15 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         if (ok && C::kOwnP && j + 1 < n) scores(j + 1);
         if (!ok) break;
         tc_fence_after();
-        if (issuer<E>(lane)) {
-          mma_cols(tmem + 128, tmem + C::kColP, smem_u32(sV + s * C::kTile), id_o, j > 0);
-          umma_commit(&v_empty[s]);
-          if (C::kOwnP) umma_commit(pv_done);
-          if (j + 1 == n) umma_commit(o_full);
+        {
+          const uint32_t v_addr = uniform<E>(smem_u32(sV + s * C::kTile)), su = uniform<E>(s);
+          const uint32_t more = uniform<E>(j > 0), last = uniform<E>(j + 1 == n);
+          if (issuer<E>(lane)) {
+            mma_cols<E>(tmem + 128, tmem + C::kColP, v_addr, id_o, more);
+            umma_commit(&v_empty[su]);
+            if (C::kOwnP) umma_commit(pv_done);
+            if (last) umma_commit(o_full);
+          }
         }
         __syncwarp();
         if (!C::kOwnP && j + 1 < n) {

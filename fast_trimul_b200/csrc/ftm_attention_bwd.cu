@@ -215,7 +215,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
   } else if (warp == kMmaWarp) {
     constexpr uint32_t id_s = idesc_f16(IsBf16<T>::v, 128, 128, 0, 0);
     constexpr uint32_t id_o = idesc_f16(IsBf16<T>::v, 128, DP, 0, 1);
-    const uint32_t q_addr = smem_u32(sQ), g_addr = smem_u32(sG);
+    const uint32_t q_addr = uniform<E>(smem_u32(sQ)), g_addr = uniform<E>(smem_u32(sG));
     int qn = 0, kn = 0;
     bool ok = true;
     // scores of key tile number i (of all this block meets); rows of K that are not keys of
@@ -238,9 +238,10 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
         __syncwarp();
       }
       tc_fence_after();
+      const uint32_t odd = uniform<E>(i & 1), k_addr = uniform<E>(smem_u32(sK + s * C::kTile));
       if (issuer<E>(lane)) {
-        mma_rows<E>(tmem + (i & 1 ? 384 : 0), q_addr, smem_u32(sK + s * C::kTile), id_s, a.ksteps);
-        umma_commit(&s_full[i & 1]);
+        mma_rows<E>(tmem + odd * 384, q_addr, k_addr, id_s, a.ksteps);
+        umma_commit(&s_full[odd]);
       }
       __syncwarp();
       return true;
@@ -249,10 +250,11 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       const int s = i % C::kV;
       if (!mbar_wait_warp(&v_full[s], (i / C::kV) & 1, a.err, err_code(KERNEL_DQ, ROLE_MMA, 3))) return false;
       tc_fence_after();
+      const uint32_t su = uniform<E>(s), v_addr = uniform<E>(smem_u32(sV + s * C::kTile));
       if (issuer<E>(lane)) {
-        mma_rows<E>(tmem + 128, g_addr, smem_u32(sV + s * C::kTile), id_s, a.ksteps);
+        mma_rows<E>(tmem + 128, g_addr, v_addr, id_s, a.ksteps);
         umma_commit(dp_full);
-        umma_commit(&v_empty[s]);
+        umma_commit(&v_empty[su]);
       }
       __syncwarp();
       return true;
@@ -268,11 +270,12 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
         if (ok && j + 1 < tiles) ok = weights_grad(kn + 1);
         if (!ok) break;
         tc_fence_after();
+        const uint32_t s = uniform<E>(kn % C::kK), odd = uniform<E>(kn & 1), more = uniform<E>(j > 0);
+        const uint32_t k_addr = uniform<E>(smem_u32(sK + s * C::kTile)), last = uniform<E>(j + 1 == tiles);
         if (issuer<E>(lane)) {
-          const int s = kn % C::kK;
-          mma_cols(tmem + 256, tmem + (kn & 1 ? 384 : 0), smem_u32(sK + s * C::kTile), id_o, j > 0);
+          mma_cols<E>(tmem + 256, tmem + odd * 384, k_addr, id_o, more);
           umma_commit(&k_empty[s]);
-          if (j + 1 == tiles) {
+          if (last) {
             umma_commit(acc_full);
             umma_commit(q_empty);
           }
@@ -526,7 +529,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   } else if (warp == kMmaWarp) {
     constexpr uint32_t id_s = idesc_f16(IsBf16<T>::v, 128, 128, 0, 0);
     constexpr uint32_t id_o = idesc_f16(IsBf16<T>::v, 128, DP, 0, 1);
-    const uint32_t k_addr = smem_u32(sK), v_addr = smem_u32(sV);
+    const uint32_t k_addr = uniform<E>(smem_u32(sK)), v_addr = uniform<E>(smem_u32(sV));
     int in = 0, qn = 0;
     bool ok = true;
     // waits for a tile of Q or g; rows behind the sequence's end are cleared, since their zero
@@ -550,13 +553,16 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       ++in;
       for (int j = -1; ok && j < tiles; ++j) {
         // (j = -1: only the first tile's scores)
-        const int i = qn + j, s = i & 1;
+        const int i = qn + j;
+        const uint32_t s = uniform<E>(i & 1), t = uniform<E>((i + 1) & 1), more = uniform<E>(j > 0);
+        const uint32_t g_at = uniform<E>(smem_u32(sG + s * C::kTile)), q_at = uniform<E>(smem_u32(sQ + s * C::kTile));
+        const uint32_t g_next = uniform<E>(smem_u32(sG + t * C::kTile)), q_next = uniform<E>(smem_u32(sQ + t * C::kTile));
         if (j >= 0) {
           ok = mbar_wait_warp(p_ready, i & 1, a.err, err_code(KERNEL_DKV, ROLE_MMA, 2));
           if (!ok) break;
           tc_fence_after();
           if (issuer<E>(lane)) {
-            mma_cols(tmem + 256, tmem, smem_u32(sG + s * C::kTile), id_o, j > 0);
+            mma_cols<E>(tmem + 256, tmem, g_at, id_o, more);
             umma_commit(&g_empty[s]);
           }
           __syncwarp();
@@ -565,7 +571,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           ok = arrived(q_full, sQ, i + 1, it.kt0 + j + 1, 3);
           if (!ok) break;
           if (issuer<E>(lane)) {
-            mma_rows<E>(tmem, k_addr, smem_u32(sQ + ((i + 1) & 1) * C::kTile), id_s, a.ksteps);
+            mma_rows<E>(tmem, k_addr, q_next, id_s, a.ksteps);
             umma_commit(s_full);
           }
           __syncwarp();
@@ -575,7 +581,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           if (!ok) break;
           tc_fence_after();
           if (issuer<E>(lane)) {
-            mma_cols(tmem + 384, tmem + 128, smem_u32(sQ + s * C::kTile), id_o, j > 0);
+            mma_cols<E>(tmem + 384, tmem + 128, q_at, id_o, more);
             umma_commit(&q_empty[s]);
           }
           __syncwarp();
@@ -584,7 +590,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           ok = arrived(g_full, sG, i + 1, it.kt0 + j + 1, 5);
           if (!ok) break;
           if (issuer<E>(lane)) {
-            mma_rows<E>(tmem + 128, v_addr, smem_u32(sG + ((i + 1) & 1) * C::kTile), id_s, a.ksteps);
+            mma_rows<E>(tmem + 128, v_addr, g_next, id_s, a.ksteps);
             umma_commit(dp_full);
           }
           __syncwarp();
@@ -811,26 +817,29 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
       if (in) mbar_wait_drain(b_full, (in - 1) & 1);
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
-      constexpr uint32_t id_s = idesc_f16(IsBf16<T>::v, 128, 128, 0, 0);
-      int rn = 0;
-      bool ok = true;
-      for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-        item(i);
-        for (int r = r0; r < r1; ++r, ++rn) {
-          const int s = rn % NS, tb = rn & 1;
-          ok = mbar_wait(&full[s], (rn / NS) & 1, a.err, err_code(KERNEL_DBIAS, ROLE_MMA, 1)) &&
-               mbar_wait(&t_empty[tb], ((rn >> 1) & 1) ^ 1, a.err, err_code(KERNEL_DBIAS, ROLE_MMA, 2));
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t st = smem_u32(smem + s * C::kStage);
+    constexpr uint32_t id_s = idesc_f16(IsBf16<T>::v, 128, 128, 0, 0);
+    int rn = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+      item(i);
+      for (int r = r0; r < r1; ++r, ++rn) {
+        const uint32_t s = uniform<E>(rn % NS), tb = uniform<E>(rn & 1);
+        const uint32_t st = uniform<E>(smem_u32(smem + s * C::kStage));
+        ok = mbar_wait_warp(&full[s], (rn / NS) & 1, a.err, err_code(KERNEL_DBIAS, ROLE_MMA, 1)) &&
+             mbar_wait_warp(&t_empty[tb], ((rn >> 1) & 1) ^ 1, a.err, err_code(KERNEL_DBIAS, ROLE_MMA, 2));
+        if (!ok) break;
+        tc_fence_after();
+        if (issuer<E>(lane)) {
           mma_rows<E>(tmem + tb * 256, st, st + 2 * C::kTile, id_s, a.ksteps);
           mma_rows<E>(tmem + tb * 256 + 128, st + C::kTile, st + 3 * C::kTile, id_s, a.ksteps);
           umma_commit(&t_full[tb]);
           umma_commit(&empty[s]);
         }
+        __syncwarp();
       }
-      if (!ok) report_failure(a);
+    }
+    if (!ok) report_failure(a);
+    if (issuer<E>(lane)) {
       umma_commit(drain);
       mbar_wait_drain(drain, 0);
     }
