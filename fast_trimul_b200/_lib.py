@@ -143,6 +143,7 @@ SIGNATURES = {
                                           _i32, _vp, _sz, _i64, _i32, _vp]),
     "ftm_attention_workspace_bytes": (_sz, [_PA, _i32]),
     "ftm_attention_fwd": (ctypes.c_int, [_PA, _i32, _vp, _sz, _vp, _vp, _vp]),
+    "ftm_pad_rows": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _vp]),
     "ftm_attention_bwd_workspace_bytes": (_sz, [_PA, _i32]),
     "ftm_attention_bwd": (ctypes.c_int, [_PA, _vp, _i64, _i64, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
@@ -235,7 +236,7 @@ def torch_ext():
         ext.bind_library([ctypes.cast(getattr(lib, name), _vp).value for name in (
             "ftm_layer_norm_fwd", "ftm_layer_norm_bwd", "ftm_layer_norm_bwd_workspace_bytes",
             "ftm_attention_fwd", "ftm_attention_bwd", "ftm_attention_workspace_bytes",
-            "ftm_attention_bwd_workspace_bytes", "ftm_last_launch_count", "ftm_status_string")])
+            "ftm_attention_bwd_workspace_bytes", "ftm_last_launch_count", "ftm_status_string", "ftm_pad_rows")])
         _torch_ext = ext
     return _torch_ext
 

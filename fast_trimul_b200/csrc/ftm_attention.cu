@@ -700,6 +700,45 @@ attn_lists_kernel(const __grid_constant__ AttnArgs a, int2* q_list, int q_cap, i
   grid_dep_release();
 }
 
+// Rows of `cols` 16-bit elements, any distance apart, to rows a multiple of 8 elements apart
+// (16-byte aligned): a thread makes 8 elements of a destination row from the aligned words
+// around them. Elements past `cols` are whatever follows, never read by the copies of the
+// kernels above, whose maps end at `cols`.
+__global__ void __launch_bounds__(256)
+pad_rows_kernel(const uint16_t* __restrict__ src, long long src_stride, uint4* __restrict__ dst, int dst_vecs,
+                long long rows, int cols) {
+  grid_dep_wait();
+  const long long n = rows * dst_vecs;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < n;
+       i += static_cast<long long>(gridDim.x) * 256) {
+    const long long r = i / dst_vecs;
+    const int c = static_cast<int>(i - r * dst_vecs) * 8;
+    const uint16_t* p = src + r * src_stride + c;
+    uint32_t w[4];
+    if (c + 8 < cols) {     // the word behind the 8 elements still belongs to the row
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(3));
+      if (reinterpret_cast<uintptr_t>(p) & 2) {
+        uint32_t x = q[0];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t y = q[k + 1];
+          w[k] = __funnelshift_r(x, y, 16);
+          x = y;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = q[k];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k] = (c + 2 * k < cols ? p[2 * k] : 0u) | ((c + 2 * k + 1 < cols ? p[2 * k + 1] : 0u) << 16);
+    }
+    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  grid_dep_release();
+}
+
 template <int DP, bool BIAS, typename T>
 cudaError_t go_fwd(const AttnLaunch& l) {
   auto kern = attn_fwd_kernel<DP, BIAS, T>;
@@ -742,6 +781,14 @@ cudaError_t launch_attn_combine(const AttnLaunch& l, int grid_fwd) {
                   : launch_pdl(attn_combine_kernel<64, __half>, grid, dim3(64), 0, l.stream, nullptr, 0, l.a, grid_fwd);
   return l.bf16 ? launch_pdl(attn_combine_kernel<128, __nv_bfloat16>, grid, dim3(128), 0, l.stream, nullptr, 0, l.a, grid_fwd)
                 : launch_pdl(attn_combine_kernel<128, __half>, grid, dim3(128), 0, l.stream, nullptr, 0, l.a, grid_fwd);
+}
+
+cudaError_t launch_pad_rows(const void* src, long long src_stride, void* dst, long long dst_stride, long long rows,
+                            int cols, int sms, cudaStream_t stream) {
+  const long long need = (rows * (dst_stride / 8) + 255) / 256, cap = static_cast<long long>(sms) * 8;
+  return launch_pdl(pad_rows_kernel, dim3(static_cast<unsigned>(need < cap ? need : cap)), dim3(256), 0, stream,
+                    nullptr, 0, static_cast<const uint16_t*>(src), src_stride, static_cast<uint4*>(dst),
+                    static_cast<int>(dst_stride / 8), rows, cols);
 }
 
 cudaError_t launch_attn_lists(const AttnLaunch& l, int2* q_list, int q_cap, int2* k_list, int k_cap,

@@ -362,6 +362,8 @@ cudaError_t launch_attn_fwd(const AttnLaunch& l);
 cudaError_t launch_attn_combine(const AttnLaunch& l, int grid_fwd);
 cudaError_t launch_attn_lists(const AttnLaunch& l, int2* q_list, int q_cap, int2* k_list, int k_cap,
                               int* counts);
+cudaError_t launch_pad_rows(const void* src, long long src_stride, void* dst, long long dst_stride, long long rows,
+                            int cols, int sms, cudaStream_t stream);
 cudaError_t launch_attn_delta(const AttnLaunch& l);
 cudaError_t launch_attn_dq(const AttnLaunch& l);
 cudaError_t launch_attn_dkv(const AttnLaunch& l);

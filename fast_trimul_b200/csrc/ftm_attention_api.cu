@@ -243,6 +243,22 @@ int ftm_attention_fwd(const ftm_attention* p, int32_t train, void* workspace, si
   return FTM_OK;
 }
 
+int ftm_pad_rows(const void* src, int64_t src_stride, void* dst, int64_t dst_stride, int64_t rows, int32_t cols,
+                 ftm_stream_t stream) {
+  set_last_launch_count(0);
+  if (!src || !dst) return FTM_BAD_ARGUMENT;
+  if (rows < 1 || cols < 1 || src_stride < cols || dst_stride < cols || dst_stride % 8 || dst_stride > (1 << 30))
+    return FTM_BAD_SHAPE;
+  if (!aligned(src, 2) || !aligned(dst, 16)) return FTM_BAD_ALIGN;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || ftm_device_supported(dev) != 1) return FTM_UNSUPPORTED_ARCH;
+  if (launch_pad_rows(src, src_stride, dst, dst_stride, rows, cols, device_sms(dev),
+                      reinterpret_cast<cudaStream_t>(stream)) != cudaSuccess)
+    return FTM_LAUNCH_FAILED;
+  set_last_launch_count(1);
+  return FTM_OK;
+}
+
 size_t ftm_attention_bwd_workspace_bytes(const ftm_attention* p, int32_t want_dbias) {
   if (check(p) != FTM_OK || p->kv_lengths) return 0;
   int dev = 0, sms = 148;

@@ -737,8 +737,10 @@ struct DbCfg {
   static constexpr int kStages = DP == 64 ? 2 : 1;
   static constexpr int kStage = 4 * kTile;    // Q, g, K, V
   static constexpr int kOffB = kStages * kStage;
-  static constexpr int kOffBar = kOffB + 2 * kBlk;
+  static constexpr int kOffT = kOffB + 2 * kBlk;          // a tile of 32 rows x 16 columns per warp
+  static constexpr int kOffBar = kOffT + kElemWarps * 32 * 17 * 4;
   static constexpr int kSmem = kOffBar + 256 + 1024;
+  static_assert(kSmem <= 232448, "dbias exceeds 227 KB of shared memory");
 };
 
 template <int DP, typename T>
@@ -899,16 +901,26 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
       if (!ok) break;
       __syncwarp();
       if (lane == 0) mbar_arrive(b_empty);
-      if (live) {
-        const size_t at = ((static_cast<size_t>(bb) * a.heads + head) * a.q_len + pos) * a.k_len;
-        const size_t all = static_cast<size_t>(biases) * a.heads * a.q_len * a.k_len;
+      // transposed in shared memory, so that 16 lanes write neighbours of a row: each lane
+      // writing along its own row cost a sector per element (16 heads of N = 1001: 340 us)
+      float* tile = reinterpret_cast<float*>(smem + C::kOffT) + warp * 32 * 17;
+      const int row0 = qt * kTileRows + quad * 32, rows = min(32, a.q_len - row0);
+      const size_t all = static_cast<size_t>(biases) * a.heads * a.q_len * a.k_len;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const int col = kt * kTileRows + part * 32 + e;
-          if (col >= a.k_len) break;
-          if (a.splits == 1) static_cast<T*>(a.dbias)[at + col] = T(acc[e]);
-          else a.dbias_part[split * all + at + col] = acc[e];
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) tile[lane * 17 + e] = acc[q * 16 + e];
+        __syncwarp();
+        const int col = kt * kTileRows + part * 32 + q * 16 + (lane & 15);
+        if (col < a.k_len) {
+          for (int y = lane >> 4; y < rows; y += 2) {
+            const size_t at = ((static_cast<size_t>(bb) * a.heads + head) * a.q_len + row0 + y) * a.k_len + col;
+            const float v = tile[y * 17 + (lane & 15)];
+            if (a.splits == 1) static_cast<T*>(a.dbias)[at] = T(v);
+            else a.dbias_part[split * all + at] = v;
+          }
         }
+        __syncwarp();
       }
     }
   }

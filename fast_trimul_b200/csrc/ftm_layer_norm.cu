@@ -11,7 +11,7 @@
 // registers and the backward's dw / db are per-thread sums: reduced per block, written as
 // one partial row per block, and added up over the blocks in a fixed order by a second
 // kernel -- no atomics, the same bits on every run. Elements per thread stay at 16 or less
-// (five such arrays in the backward), which keeps 128 registers and 2-4 blocks per SM.
+// (five such arrays in the backward), which keeps 64 to 128 registers and 2-4 blocks per SM.
 // Loads are 16 bytes where width, stride and pointers allow it, else 4 bytes or one element.
 // Widths beyond 8192 take a plain block-per-row loop that re-reads the row from cache.
 #include "ftm_kernels.h"
@@ -156,7 +156,8 @@ ln_fwd_kernel(const T* __restrict__ x, long long xs, const void* __restrict__ w,
 // dx (null: not wanted) and, where `partial` is given, this block's sums of g h and g as
 // partial[block][2][width]
 template <typename T, int VEC, int TPR, int ITER, int R>
-__global__ void __launch_bounds__(TPR > 32 ? TPR : kLnThreads)
+__global__ void __launch_bounds__(TPR > 32 ? TPR : kLnThreads,
+                                  (ITER * VEC <= 8 ? 1024 : 512) / (TPR > 32 ? TPR : kLnThreads))
 ln_bwd_kernel(const T* __restrict__ x, long long xs, const T* __restrict__ g, long long gs,
               const void* __restrict__ w, int wdt, const float2* __restrict__ stats,
               T* __restrict__ dx, float* __restrict__ partial, long long rows, int width) {
@@ -415,10 +416,11 @@ template <typename T, int VEC, int TPR, int ITER>
 cudaError_t ln_go(LnArgs& a, bool bwd) {
   constexpr int E = VEC * ITER;
   constexpr int kBlock = TPR > 32 ? TPR : kLnThreads;
-  // rows in flight per group: enough bytes in flight for a bandwidth-bound loop when a
-  // row is only a few elements per thread
+  // rows in flight per group: 1048576 x 128 bf16 forward took 131 / 112 / 109 us with 1 / 2 / 4
+  // rows (4.9 TB/s); backward 159 us with one row in 64 registers and four blocks per SM
+  // (5.1 TB/s) against 212 and 398 us with 2 and 4 rows, whose registers spill
   constexpr int RF = TPR > 32 ? (E <= 8 ? 2 : 1) : (E <= 2 ? 4 : E <= 8 ? 4 : 2);
-  constexpr int RB = TPR > 32 ? 1 : (E <= 8 ? 2 : 1);
+  constexpr int RB = 1;
   if (!bwd) {
     const int blocks = ln_blocks(a.rows, kBlock / TPR * RF, kBlock, a.sms, false);
     return launch_pdl(ln_fwd_kernel<T, VEC, TPR, ITER, RF>, dim3(blocks), dim3(kBlock), 0, a.stream,

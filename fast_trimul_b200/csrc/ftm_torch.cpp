@@ -34,6 +34,7 @@ struct Library {
   decltype(&ftm_attention_bwd_workspace_bytes) at_bwd_bytes = nullptr;
   decltype(&ftm_last_launch_count) launches = nullptr;
   decltype(&ftm_status_string) status = nullptr;
+  decltype(&ftm_pad_rows) pad_rows = nullptr;
 } lib;
 
 // error words of each GPU: the device word and the pinned host word (see ops/attention.py)
@@ -401,7 +402,14 @@ py::object pair(const Tensor& q, const Tensor& k, const Tensor& v, const OptTens
     if (!ready(b)) {
       const int64_t wide = (N + 7) / 8 * 8;
       rb = at::empty({b.size(0), H, N, wide}, q.options().memory_format(at::MemoryFormat::Contiguous)).slice(3, 0, N);
-      rb.copy_(b.detach());
+      if (b.is_contiguous()) {
+        const c10::cuda::OptionalCUDAGuard guard(q.device());
+        check(lib.pad_rows(b.data_ptr(), N, rb.data_ptr(), wide, b.size(0) * H * N, static_cast<int>(N), stream_of(q)),
+              "ftm_pad_rows");
+        count(false);
+      } else {
+        rb.copy_(b.detach());
+      }
     }
   }
   if (B * R * N > INT_MAX) return py::none();
@@ -419,7 +427,7 @@ py::object pair(const Tensor& q, const Tensor& k, const Tensor& v, const OptTens
 }
 
 void bind_library(const std::vector<uintptr_t>& f) {
-  TORCH_CHECK(f.size() == 9, "nine functions");
+  TORCH_CHECK(f.size() == 10, "ten functions");
   int i = 0;
   const auto set = [&](auto& p) { p = reinterpret_cast<std::decay_t<decltype(p)>>(f[i++]); };
   set(lib.ln_fwd);
@@ -431,6 +439,7 @@ void bind_library(const std::vector<uintptr_t>& f) {
   set(lib.at_bwd_bytes);
   set(lib.launches);
   set(lib.status);
+  set(lib.pad_rows);
 }
 
 void set_words(int device, uintptr_t dev, uintptr_t host) {

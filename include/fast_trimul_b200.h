@@ -394,6 +394,12 @@ size_t ftm_attention_workspace_bytes(const ftm_attention* p, int32_t train);
 int ftm_attention_fwd(const ftm_attention* p, int32_t train, void* workspace, size_t workspace_bytes,
                       int* err_word, int* host_word, ftm_stream_t stream);
 
+/* Copies rows of `cols` 16-bit elements, src_stride elements apart (at least cols), to rows
+ * dst_stride elements apart (a multiple of 8, dst 16-byte aligned): a bias whose row length is
+ * no multiple of 8 as the attention calls want it. Elements behind cols are undefined. */
+int ftm_pad_rows(const void* src, int64_t src_stride, void* dst, int64_t dst_stride, int64_t rows, int32_t cols,
+                 ftm_stream_t stream);
+
 /* Backward (not of the cache form): p as in the forward, with its out and stats, and the
  * forward's workspace (train = 1). grad: (q_rows, heads, head_dim), its strides in elements.
  * dq like out; dk, dv contiguous (kv_rows, kv_heads, head_dim); dbias contiguous

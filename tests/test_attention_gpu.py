@@ -629,3 +629,20 @@ def test_fused_trunk_trains():
     for k, want in grads[0].items():
         # a chain of some 30 bf16 roundings of 2^-9 each; small gradients ride on large terms
         assert (grads[1][k] - want).norm() <= 0.1 * want.norm() + 1e-5, k
+
+
+@pytest.mark.parametrize("cols", [1, 2, 7, 8, 9, 15, 16, 17, 31, 33, 250, 1001])
+@pytest.mark.parametrize("shift", [0, 1, 2, 3])
+def test_pad_rows_copies_every_element(cols, shift):
+    """Rows at every alignment, the last one ending with its buffer."""
+    from fast_trimul_b200 import _lib
+    lib = _lib.load()
+    rows, wide = 13, (cols + 7) // 8 * 8
+    buf = torch.arange(rows * cols + shift, device="cuda").to(torch.int16)
+    src = buf[shift:].view(rows, cols)
+    dst = torch.full((rows, wide), -1, dtype=torch.int16, device="cuda")
+    s = torch.cuda.current_stream().cuda_stream
+    assert lib.ftm_pad_rows(src.data_ptr(), cols, dst.data_ptr(), wide, rows, cols, s) == _lib.OK
+    assert torch.equal(dst[:, :cols], src)
+    assert lib.ftm_pad_rows(src.data_ptr(), cols - 1, dst.data_ptr(), wide, rows, cols, s) == _lib.BAD_SHAPE
+    assert lib.ftm_pad_rows(src.data_ptr(), cols, dst.data_ptr(), wide + 1, rows, cols, s) == _lib.BAD_SHAPE
