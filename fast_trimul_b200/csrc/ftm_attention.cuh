@@ -36,6 +36,8 @@ struct AttnArgs {
   const uint8_t* key_mask;   // one byte per key row, 0: not seen; may be null
   int bias_seqs;             // consecutive sequences that share a bias
   int splits;                // bias gradient: parts of those sequences
+  int kv_splits;             // dk, dv: parts of the query tiles of a key tile
+  float* dkv_part;           // their partial sums: [part][dk, dv][row][kv head][dim]
   // outputs and operands that are read by plain loads; contiguous unless strides follow
   void* out;
   const void* o;             // forward output (backward)
@@ -136,7 +138,7 @@ __device__ __forceinline__ void kv_item(const AttnArgs& a, int seq, int tile, in
 }
 
 template <bool KV>
-__device__ __forceinline__ bool walk_item(const AttnArgs& a, int n, Item& it) {
+__device__ __forceinline__ bool walk_item_whole(const AttnArgs& a, int n, Item& it) {
   if (a.walk == WALK_LIST) {
     const int w = n / a.kv_heads;
     if (w >= *a.count) return false;
@@ -151,6 +153,20 @@ __device__ __forceinline__ bool walk_item(const AttnArgs& a, int n, Item& it) {
   if (KV) kv_item(a, rest / a.kv_heads, n % tiles, rest % a.kv_heads, it);
   else q_item(a, rest / a.kv_heads, n % tiles, rest % a.kv_heads, it);
   return true;
+}
+
+template <bool KV>
+__device__ __forceinline__ bool walk_item(const AttnArgs& a, int n, Item& it) {
+  if (KV && a.kv_splits > 1) {   // the parts of an item are neighbours
+    const int part = n % a.kv_splits;
+    if (!walk_item_whole<KV>(a, n / a.kv_splits, it)) return false;
+    const int t = it.kt1 - it.kt0, t0 = it.kt0;
+    it.kt0 = t0 + t * part / a.kv_splits;
+    it.kt1 = t0 + t * (part + 1) / a.kv_splits;
+    it.slot = part;
+    return true;
+  }
+  return walk_item_whole<KV>(a, n, it);
 }
 
 // ------------------------------------------------------------------- tcgen05 forms
@@ -367,6 +383,7 @@ cudaError_t launch_pad_rows(const void* src, long long src_stride, void* dst, lo
 cudaError_t launch_attn_delta(const AttnLaunch& l);
 cudaError_t launch_attn_dq(const AttnLaunch& l);
 cudaError_t launch_attn_dkv(const AttnLaunch& l);
+cudaError_t launch_attn_dkv_reduce(const AttnLaunch& l);
 cudaError_t launch_attn_dbias(const AttnLaunch& l);
 int attn_fwd_grid(const AttnLaunch& l);
 

@@ -124,14 +124,29 @@ FwdSpace fwd_space(const ftm_attention* p, int train, int sms) {
   return w;
 }
 
-// backward: [row constants][parts of the bias gradient]
+// backward: [row constants][parts of dk and dv][parts of the bias gradient]
 struct BwdSpace {
-  size_t part, total;
-  int splits;
+  size_t kv_part, part, total;
+  int splits, kv_splits;
 };
 BwdSpace bwd_space(const ftm_attention* p, int want_dbias, int sms) {
   BwdSpace w{};
-  w.part = up256(size_t(p->q_rows) * p->heads * sizeof(float4));
+  w.kv_part = up256(size_t(p->q_rows) * p->heads * sizeof(float4));
+  w.part = w.kv_part;
+  // Few key tiles (one key / value head, a few thousand keys) leave SMs idle: the query tiles of
+  // each are split over up to 8 blocks, at least 4 tiles each, and the parts added up. One
+  // sequence of 2319 tokens, 8 heads on one, dim 128: the dkv kernel 263 us unsplit, 66 us with
+  // the parts' sums.
+  const int64_t tq = kTileRows / (p->heads / p->kv_heads);
+  const int64_t k_items = (p->cu_q ? p->kv_rows / kTileRows + p->sequences
+                                   : int64_t(p->sequences) * ((p->kv_len + kTileRows - 1) / kTileRows)) * p->kv_heads;
+  const int64_t q_tiles = (p->q_rows / p->sequences + tq - 1) / tq;
+  int64_t ks = sms / (k_items > 0 ? k_items : 1);
+  if (ks > 8) ks = 8;
+  if (ks > q_tiles / 4) ks = q_tiles / 4;
+  w.kv_splits = ks < 2 ? 1 : static_cast<int>(ks);
+  if (w.kv_splits > 1)
+    w.part += up256(size_t(2) * w.kv_splits * p->kv_rows * p->kv_heads * p->head_dim * sizeof(float));
   w.total = w.part;
   w.splits = 1;
   if (want_dbias && p->bias) {
@@ -180,6 +195,7 @@ bool fill(AttnLaunch& l, const ftm_attention* p, int dev, int* err, int* host_er
   a.k_lens = p->kv_lengths;
   a.key_mask = p->key_mask;
   a.bias_seqs = p->bias ? p->bias_seqs : 1;
+  a.splits = a.kv_splits = 1;
   a.out = p->out;
   a.stats = reinterpret_cast<float2*>(p->stats);
   a.err = err;
@@ -305,6 +321,8 @@ int ftm_attention_bwd(const ftm_attention* p, const void* grad, int64_t grad_row
   l.a.dbias = dbias;
   l.a.dbias_part = reinterpret_cast<float*>(ws + w.part);
   l.a.splits = w.splits;
+  l.a.kv_splits = w.kv_splits;
+  l.a.dkv_part = reinterpret_cast<float*>(ws + w.kv_part);
   int launches = 1;
   if (launch_attn_delta(l) != cudaSuccess) return FTM_LAUNCH_FAILED;
   uint8_t* lists = static_cast<uint8_t*>(fwd_workspace);
@@ -323,6 +341,10 @@ int ftm_attention_bwd(const ftm_attention* p, const void* grad, int64_t grad_row
     }
     if (launch_attn_dkv(l) != cudaSuccess) return FTM_LAUNCH_FAILED;
     ++launches;
+    if (w.kv_splits > 1) {
+      if (launch_attn_dkv_reduce(l) != cudaSuccess) return FTM_LAUNCH_FAILED;
+      ++launches;
+    }
   }
   if (dbias) {
     if (launch_attn_dbias(l) != cudaSuccess) return FTM_LAUNCH_FAILED;

@@ -102,6 +102,31 @@ __device__ __forceinline__ void store_acc(uint32_t taddr, int col0, int dim, flo
   }
 }
 
+// the same unrounded, to a row of a partial sum
+template <int COLS>
+__device__ __forceinline__ void store_part(uint32_t taddr, int col0, int dim, float f, bool live, bool any, float* out) {
+#pragma unroll
+  for (int q = 0; q < COLS / 16; ++q) {
+    uint32_t o[16];
+    if (any) {
+      tmem_ld16_nowait(taddr + col0 + q * 16, o);
+      tmem_wait_ld();
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e] = 0;
+    }
+    if (!live) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = col0 + q * 16 + e * 4;
+      if (c >= dim) break;
+      *reinterpret_cast<float4*>(out + c) =
+          make_float4(__uint_as_float(o[e * 4]) * f, __uint_as_float(o[e * 4 + 1]) * f,
+                      __uint_as_float(o[e * 4 + 2]) * f, __uint_as_float(o[e * 4 + 3]) * f);
+    }
+  }
+}
+
 // the bits of key_bits() for this warp's 32 columns of tile kt
 __device__ __forceinline__ uint32_t key_word(const AttnArgs& a, const Item& it, int kt, int part, int lane) {
   const int c = kt * kTileRows + part * 32 + lane;
@@ -613,7 +638,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float c = log2_scale(a.scale);
     T *dk = static_cast<T*>(a.dk), *dv = static_cast<T*>(a.dv);
-    if (a.walk == WALK_LIST) {
+    if (a.walk == WALK_LIST && a.kv_splits == 1) {
       const long long per = static_cast<long long>(a.kv_heads) * a.dim / 8;
       zero_outside(a.cu_k, a.seqs, a.kv_rows, per, dk, threadIdx.x, kElemWarps * 32);
       zero_outside(a.cu_k, a.seqs, a.kv_rows, per, dv, threadIdx.x, kElemWarps * 32);
@@ -718,8 +743,15 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         ++in;
         tc_fence_after();
       }
-      store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, 1.f, live, any, dv + orow * a.dim);
-      store_acc<DP / 4>(lanes + 384, part * (DP / 4), a.dim, a.scale, live, any, dk + orow * a.dim);
+      if (a.kv_splits > 1) {
+        const size_t all = static_cast<size_t>(a.kv_rows) * a.kv_heads * a.dim;
+        float* to = a.dkv_part + 2 * it.slot * all + orow * a.dim;
+        store_part<DP / 4>(lanes + 384, part * (DP / 4), a.dim, a.scale, live, any, to);
+        store_part<DP / 4>(lanes + 256, part * (DP / 4), a.dim, 1.f, live, any, to + all);
+      } else {
+        store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, 1.f, live, any, dv + orow * a.dim);
+        store_acc<DP / 4>(lanes + 384, part * (DP / 4), a.dim, a.scale, live, any, dk + orow * a.dim);
+      }
       tc_fence_before();
     }
   }
@@ -931,6 +963,34 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
   if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
+// dk and dv = sums of the parts, in order; rows of no sequence, which no part wrote, are zero
+template <typename T>
+__global__ void __launch_bounds__(256)
+attn_dkv_reduce_kernel(const __grid_constant__ AttnArgs a) {
+  grid_dep_wait();
+  const long long per = static_cast<long long>(a.kv_heads) * a.dim, all = per * a.kv_rows;
+  int lo = 0, hi = a.kv_rows;
+  if (a.walk == WALK_LIST) {
+    lo = min(max(a.cu_k[0], 0), a.kv_rows);
+    hi = min(max(a.cu_k[a.seqs], lo), a.kv_rows);
+  }
+  for (long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 4; i < 2 * all;
+       i += static_cast<long long>(gridDim.x) * 1024) {
+    const bool second = i >= all;
+    const long long e = second ? i - all : i;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    const long long row = e / per;
+    if (row >= lo && row < hi)
+      for (int k = 0; k < a.kv_splits; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(a.dkv_part + 2 * k * all + i);
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+      }
+    *reinterpret_cast<uint2*>(static_cast<T*>(second ? a.dv : a.dk) + e) =
+        make_uint2(pack16<T>(s.x, s.y), pack16<T>(s.z, s.w));
+  }
+  grid_dep_release();
+}
+
 // dbias = sum of the splits' parts, in order
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -952,6 +1012,7 @@ int item_grid(const AttnLaunch& l, bool kv) {
                  : (static_cast<long long>(a.q_rows) + a.tq - 1) / a.tq) + a.seqs) * a.kv_heads;
   else
     items = static_cast<long long>(a.seqs) * (kv ? a.k_tiles : a.q_tiles) * a.kv_heads;
+  if (kv) items *= a.kv_splits;
   return static_cast<int>(items < l.sms ? items : l.sms);
 }
 
@@ -991,6 +1052,14 @@ cudaError_t launch_attn_dkv(const AttnLaunch& l) {
   const int grid = item_grid(l, true);
 #define DKV_SMEM(D, B) (DkvCfg<D, B>::kSmem)
   FTM_BY_SHAPE(attn_dkv_kernel, DKV_SMEM, grid)
+}
+
+cudaError_t launch_attn_dkv_reduce(const AttnLaunch& l) {
+  const long long n = static_cast<long long>(l.a.kv_rows) * l.a.kv_heads * l.a.dim / 2;   // float4s of both
+  const long long need = (n + 255) / 256, cap = static_cast<long long>(l.sms) * 8;
+  const dim3 grid(static_cast<unsigned>(need < cap ? need : cap));
+  if (l.bf16) return launch_pdl(attn_dkv_reduce_kernel<__nv_bfloat16>, grid, dim3(256), 0, l.stream, nullptr, 0, l.a);
+  return launch_pdl(attn_dkv_reduce_kernel<__half>, grid, dim3(256), 0, l.stream, nullptr, 0, l.a);
 }
 
 cudaError_t launch_attn_dbias(const AttnLaunch& l) {

@@ -203,6 +203,19 @@ def test_packed_many_short_sequences():
     check_packed(q[a:b], k[a:b], v[a:b], part, part)
 
 
+@pytest.mark.parametrize("h,hk,lens,klens", [(8, 1, [900], [900]), (16, 1, [700, 90], [300, 900]), (8, 2, [640, 1, 513], [640, 1, 513])],
+                         ids=str)
+@pytest.mark.parametrize("causal", [False, True])
+def test_packed_few_key_tiles_split_their_queries(h, hk, lens, klens, causal):
+    """Shapes whose key tiles are too few for the GPU: parts of the queries are summed, and rows of
+    no sequence stay zero."""
+    q, k, v = qkv(sum(lens) + 9, sum(klens) + 13, h, hk, 64, BF)
+    k[sum(klens) + 5:], v[:5] = float("nan"), float("inf")
+    got = check_packed(q, k, v, ends(lens, 4), ends(klens, 5), causal)
+    for g in got[2:]:
+        assert (g[:5] == 0).all() and (g[sum(klens) + 5:] == 0).all()
+
+
 def test_gradients_against_differences():
     """The kernels' gradients along a direction against differences of the 64-bit forward."""
     cu = ends([37])
