@@ -15,6 +15,11 @@
 // special function unit, so dim 128 is balanced between the two and smaller heads are
 // bound by the exponentials.
 //
+// Measured, bf16: 2 sequences of 8192 tokens, 16 heads, dim 128, 1000 us (1100 TFLOP/s);
+// one of them, causal, 300 us (917); triangle attention at N = 384, 4 heads of 32, 149 us, the
+// exponentials alone 49; one token over 16 caches of 9000 to 16384 tokens, 8 heads of 128
+// shared by 32, 154 us (6.0 TB/s).
+//
 // Persistent grid. Packed sequences: a one-block kernel lists (sequence, tile) by
 // descending number of key tiles, so the long ones start first. Cache: the key tiles of
 // all sequences and heads are cut into equal runs, one per block; a sequence that spans

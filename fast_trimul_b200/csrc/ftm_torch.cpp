@@ -8,7 +8,9 @@
 // around it then checks, copies, runs elsewhere or raises, and may call again. The library's
 // functions come as addresses from the ctypes binding, so there is one loaded library.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <array>
@@ -73,6 +75,44 @@ void* ptr(const OptTensor& t) { return t.has_value() && t->defined() ? t->data_p
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 
+// ---------------------------------------------------------------------------- autograd
+// The gradients of a backward. With create_graph they hang on a node that raises when it is
+// differentiated in turn, `from` (what they were formed of) behind it: these operators have
+// first derivatives only, and a second one must not come out as zero.
+variable_list once(variable_list grads, const variable_list& from) {
+  const size_t n = grads.size();
+  for (Tensor& t : grads)
+    if (t.defined()) t = t.detach().set_requires_grad(true);
+  grads.insert(grads.end(), from.begin(), from.end());
+  const auto stop = std::make_shared<torch::autograd::DelayedError>(
+      "layer norm and attention of fast_trimul_b200 are differentiable once", static_cast<int64_t>(grads.size()));
+  variable_list out = (*stop)(std::move(grads));
+  out.resize(n);
+  return out;
+}
+
+bool capturing() { return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; }
+
+// A leaf whose gradients an eager graph that still lives collects on the default stream. A
+// backward pass in a captured graph would wait on that stream, which cannot take part in a
+// capture: such a backward is refused (`not_held`) while the error can still be raised.
+bool held(std::initializer_list<const Tensor*> leaves) {
+  if (!capturing()) return false;
+  for (const Tensor* t : leaves) {
+    if (!t || !t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    if (stream && stream->device_type() == at::kCUDA && !c10::cuda::CUDAStream(*stream).stream()) return true;
+  }
+  return false;
+}
+void not_held(bool held) {
+  TORCH_CHECK(!held || !capturing(),
+              "a backward pass cannot be captured while a graph made on the default stream holds the same leaves: "
+              "drop its outputs first, or run it on another stream");
+}
+const Tensor* given(const OptTensor& t) { return has(t) ? &*t : nullptr; }
+
 // -------------------------------------------------------------------------- layer norm
 // rows of `width` contiguous elements one stride apart; false: some other layout
 bool rows_of(const Tensor& t, int64_t& rows, int64_t& stride) {
@@ -111,10 +151,19 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     Tensor out = run(x, w.value_or(Tensor()), b.value_or(Tensor()), eps, &stats);
     ctx->save_for_backward({x, w.value_or(Tensor()), stats});
     ctx->saved_data["bias"] = has(b) ? static_cast<int64_t>(b->scalar_type()) : int64_t(-1);
+    ctx->saved_data["held"] = held({&x, given(w), given(b)});
     return out;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    not_held(ctx->saved_data["held"].toBool());
+    variable_list res = gradients(ctx, grads);
+    if (!at::GradMode::is_enabled()) return res;
+    const auto saved = ctx->get_saved_variables();
+    return once(std::move(res), {grads[0], saved[0], saved[1]});
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const at::AutoDispatchBelowAutograd below;
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
@@ -171,7 +220,7 @@ py::object layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, d
 // What a call is beside its tensors.
 struct Call {
   int seqs = 0, q_len = 0, kv_len = 0, bias_seqs = 0;
-  bool causal = false;
+  bool causal = false, held = false;
   double scale = 0;
   Tensor cu_q, cu_k, lengths, mask, ready_bias;
 };
@@ -261,11 +310,20 @@ struct Attention : torch::autograd::Function<Attention> {
     ctx->save_for_backward({q, k, v, c.ready_bias, out, stats, lists, c.cu_q, c.cu_k, c.mask});
     ctx->saved_data["n"] = std::vector<int64_t>{c.seqs, c.q_len, c.kv_len, c.bias_seqs, c.causal};
     ctx->saved_data["scale"] = c.scale;
+    ctx->saved_data["held"] = c.held;
     if (has(bias)) ctx->saved_data["bias"] = bias->sizes().vec();
     return out;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    not_held(ctx->saved_data["held"].toBool());
+    variable_list res = gradients(ctx, grads);
+    if (!at::GradMode::is_enabled()) return res;
+    const auto saved = ctx->get_saved_variables();
+    return once(std::move(res), {grads[0], saved[0], saved[1], saved[2]});
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const at::AutoDispatchBelowAutograd below;
     const auto s = ctx->get_saved_variables();
     const Tensor &q = s[0], &k = s[1], &v = s[2], &bias = s[3], &out = s[4], &stats = s[5], &lists = s[6];
@@ -360,6 +418,7 @@ py::object packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   c.cu_q = cu_q;
   c.cu_k = cu_k;
   if (has(mask)) c.mask = *mask;
+  c.held = held({&q, &k, &v});
   return py::cast(run(c, q, k, v, std::nullopt));
 }
 
@@ -420,6 +479,7 @@ py::object pair(const Tensor& q, const Tensor& k, const Tensor& v, const OptTens
   if (b.defined()) c.bias_seqs = static_cast<int>(B * R / b.size(0));
   if (has(mask)) c.mask = *mask;
   c.ready_bias = rb;
+  c.held = held({&q, &k, &v, given(bias)});
   const auto rows = [&](const Tensor& t) { return t.reshape({B * R * N, H, D}); };
   Tensor qf = rows(q), kf = rows(k), vf = rows(v);
   if (!ready(qf) || !ready(kf) || !ready(vf)) return py::none();

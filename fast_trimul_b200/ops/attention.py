@@ -18,6 +18,7 @@ sees no key gives zeros, and masked keys count as absent whatever K and V hold t
 
 import ctypes
 import math
+import threading
 
 import torch
 
@@ -32,10 +33,13 @@ class AttentionErrorWord:
     next call (or `check`) sees that with a plain read; no call copies or synchronises."""
 
     def __init__(self, device):
+        if torch.cuda.is_current_stream_capturing():
+            raise _lib.NativeDeclined("the first attention call on a GPU cannot be captured: warm up before the capture")
         self.dev = torch.zeros(64, dtype=torch.int32, device=device)
         self.host = torch.zeros(16, dtype=torch.int32).pin_memory()
         self.ptr, self.host_ptr = self.dev.data_ptr(), self.host.data_ptr()
         self.word = ctypes.c_int32.from_address(self.host_ptr)
+        torch.cuda.synchronize(device)     # zeroed, whatever stream reads it first
         _lib.torch_ext().set_words(self.dev.device.index, self.ptr, self.host_ptr)
 
     def poll(self):
@@ -55,6 +59,7 @@ class AttentionErrorWord:
 
 
 _ERROR_WORDS = {}
+_ERROR_WORDS_LOCK = threading.Lock()
 
 
 def attention_error_word(device=None):
@@ -62,7 +67,10 @@ def attention_error_word(device=None):
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     w = _ERROR_WORDS.get(index)
     if w is None:
-        w = _ERROR_WORDS[index] = AttentionErrorWord(torch.device("cuda", index))
+        with _ERROR_WORDS_LOCK:      # one per GPU, never replaced: kernels hold its addresses
+            w = _ERROR_WORDS.get(index)
+            if w is None:
+                w = _ERROR_WORDS[index] = AttentionErrorWord(torch.device("cuda", index))
     return w
 
 
@@ -149,6 +157,11 @@ def _attend(q, k, v, keep, scale, bias=None):
     return (p / torch.where(total == 0, torch.ones_like(total), total)) @ v
 
 
+def _nothing(like, *inputs):
+    """Zeros of `like`'s shape that depend on the inputs, whatever they hold."""
+    return torch.zeros_like(like) + sum(t[:0].sum().to(like.dtype) for t in inputs)
+
+
 # --------------------------------------------------------------------------- packed
 def _ends(cu, device, name):
     if cu.dim() != 1 or cu.numel() < 1 or cu.dtype.is_floating_point or cu.dtype == torch.bool:
@@ -175,7 +188,7 @@ def _packed_torch(q, k, v, cu_q, cu_k, causal, scale, mask):
                           t[c:d].float().masked_fill(~mask[c:d, None, None], 0)
                           ).transpose(0, 1).repeat_interleave(group, 0)
         if m == 0:
-            o = qs * 0
+            o = _nothing(qs, qs, k, v)
         else:
             o = _attend(qs, rows(k), rows(v), keep, scale)
         pieces += [out[at:a], o.transpose(0, 1)]
@@ -192,7 +205,8 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, *, causal=True, sca
     device that do not descend. Rows of no sequence give zeros. `causal`: query i of a sequence
     sees keys j <= i + (keys - queries), aligned to the last key, so a prompt's continuation
     passes its new queries and all keys. scale: dim ** -0.5 if None. key_mask: (rows of k,), keys
-    with 0 / False are not seen. Returns q's shape and type. Differentiable once in q, k and v."""
+    with 0 / False are not seen and may hold anything (keys that only `causal` hides from some
+    queries must be finite). Returns q's shape and type. Differentiable once in q, k and v."""
     if q.is_cuda and (cu_seqlens_k is not None or q.shape[0] == k.shape[0]):
         out = _native("packed", q, k, v, cu_seqlens, cu_seqlens if cu_seqlens_k is None else cu_seqlens_k,
                       bool(causal), scale, key_mask)
@@ -211,10 +225,10 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, *, causal=True, sca
     if cu_q.numel() != cu_k.numel():
         raise ValueError(f"{cu_q.numel() - 1} query sequences, {cu_k.numel() - 1} key sequences")
     mask = None if key_mask is None else _as_mask(key_mask, q.device, (k.shape[0],), "key_mask")
+    if cu_q.numel() < 2 or q.shape[0] == 0 or k.shape[0] == 0:
+        return _nothing(q, q, k, v)
     if not q.is_cuda:
         return _packed_torch(q, k, v, cu_q, cu_k, causal, s, mask)
-    if cu_q.numel() < 2 or q.shape[0] == 0 or k.shape[0] == 0:
-        return q * 0 + (k.sum() + v.sum()) * 0 if torch.is_grad_enabled() else torch.zeros_like(q)
     return _prepared("packed", _in_place(q), _in_place(k), _in_place(v), cu_q, cu_k, bool(causal), s,
                      None if mask is None else mask.contiguous())
 
@@ -280,7 +294,7 @@ def pair_attention(q, k, v, bias, mask=None, *, scale=None):
         raise ValueError(f"bias must have shape ({B} or 1, {H}, {N}, {N}), got {tuple(bias.shape)}")
     m = None if mask is None else _as_mask(mask, q.device, (B, R, N), "mask")
     if q.numel() == 0:
-        return q * 0 if bias is None else q * 0 + bias.sum() * 0
+        return _nothing(q, q, k, v, *(() if bias is None else (bias,)))
     if not q.is_cuda:
         keep = torch.ones(B, R, N, dtype=torch.bool, device=q.device) if m is None else m
         rows = lambda t: t.float().masked_fill(~keep[..., None, None], 0).transpose(2, 3)   # noqa: E731

@@ -106,6 +106,16 @@ def test_no_sequences_and_no_rows():
     assert pair_attention(r(1, 0, 4, 2, 8), r(1, 0, 4, 2, 8), r(1, 0, 4, 2, 8), r(1, 2, 4, 4)).shape == (1, 0, 4, 2, 8)
 
 
+def test_nothing_to_attend_to_gives_zeros_whatever_the_inputs_hold():
+    bad = torch.full((3, 2, 8), float("nan"), requires_grad=True)
+    for out in (packed_attention(bad, bad, bad, torch.tensor([0])),
+                packed_attention(bad, bad[:0], bad[:0], ends([3]), torch.tensor([0, 0])),
+                packed_attention(bad, bad, bad, torch.tensor([0, 3]), torch.tensor([1, 1]))):
+        assert torch.equal(out, torch.zeros_like(bad))
+        (grad,) = torch.autograd.grad(out.sum(), bad)
+        assert torch.equal(grad, torch.zeros_like(bad))
+
+
 def test_c_entry_points_check_their_arguments_before_the_device():
     lib = _lib.load()
     p = 1 << 20     # a 256-byte aligned address, never dereferenced

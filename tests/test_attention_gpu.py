@@ -550,6 +550,70 @@ def test_refusals():
             bad()
 
 
+def test_nothing_to_attend_to_gives_zeros_whatever_the_inputs_hold():
+    from fast_trimul_b200.functional import packed_attention
+    bad = torch.full((3, 2, 8), float("nan"), dtype=BF, device="cuda", requires_grad=True)
+    for out in (packed_attention(bad, bad, bad, ends([])),
+                packed_attention(bad, bad[:0], bad[:0], ends([3]), ends([0]))):
+        assert torch.equal(out, torch.zeros_like(bad))
+        (grad,) = torch.autograd.grad(out.sum(), bad)
+        assert torch.equal(grad, torch.zeros_like(bad))
+
+
+@pytest.mark.parametrize("kind", ["packed", "pair", "layer_norm"])
+def test_second_derivatives_are_refused(kind):
+    # a gradient taken with create_graph is right, and differentiating it raises
+    from fast_trimul_b200.functional import layer_norm, packed_attention, pair_attention
+    if kind == "packed":
+        leaves, f = qkv(40, 40, 4, 2, 64, BF), lambda *x: packed_attention(*x, ends([40]))
+    elif kind == "pair":
+        leaves, f = pair_inputs(1, 2, 24, 2, 32, BF), pair_attention
+    else:
+        r = gen(4)
+        leaves, f = [r(5, 64).to(BF), r(64), r(64)], layer_norm
+    leaves = [t.detach().clone().requires_grad_() for t in leaves]
+    g = gen(1)(*leaves[0].shape).to(BF)
+    want = torch.autograd.grad(f(*leaves), leaves, g)
+    got = torch.autograd.grad(f(*leaves), leaves, g, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(sum(x.float().sum() for x in got), leaves)
+    got = torch.autograd.grad(f(*leaves), leaves, g, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        sum(x.float().sum() for x in got).backward()
+
+
+@pytest.mark.parametrize("kind", ["packed", "pair", "layer_norm"])
+def test_a_captured_backward_of_leaves_that_an_eager_graph_holds_is_refused(kind):
+    from fast_trimul_b200.functional import layer_norm, packed_attention, pair_attention
+    if kind == "packed":
+        leaves, f = qkv(40, 40, 4, 2, 64, BF), lambda *x: packed_attention(*x, cu)
+        cu = ends([40])
+    elif kind == "pair":
+        leaves, f = pair_inputs(1, 2, 24, 2, 32, BF), pair_attention
+    else:
+        r = gen(4)
+        leaves, f = [r(5, 64).to(BF), r(64), r(64)], layer_norm
+    leaves = [t.detach().clone().contiguous().requires_grad_() for t in leaves]
+    g = gen(1)(*leaves[0].shape).to(BF)
+    want = torch.autograd.grad(f(*leaves), leaves, g)
+    eager = f(*leaves)                      # lives over the capture
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        with torch.cuda.graph(graph, stream=s):
+            out = f(*leaves)                # a forward may be captured
+            with pytest.raises(RuntimeError, match="cannot be captured"):
+                torch.autograd.grad(out, leaves, g)
+    torch.cuda.current_stream().wait_stream(s)
+    graph.replay()
+    assert torch.equal(out, eager)
+    got = torch.autograd.grad(eager, leaves, g)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    check_waits()
+
+
 def test_a_withheld_tile_is_reported_and_the_next_call_is_right(monkeypatch):
     """A bounded wait that expires (a test switch withholds one K tile) ends the kernel, and the
     next call raises; nothing faults, and afterwards results are right."""
