@@ -174,11 +174,13 @@ __device__ __forceinline__ float row_max(uint32_t taddr, const uint8_t* sB, int 
 
 // Weights 2^(c (t - ref)) of a row, written as 16-bit pairs to 64 columns at `paddr` (which may
 // be the scores' own first columns: those have been read by then); their sum. `before_store`
-// runs in front of the first store. FAR: the difference first (see the call).
+// runs in front of the first store, `all_read` once the last scores are in registers. FAR: the
+// difference first (see the call).
 // (A polynomial on the FMA pipe for a fourth to a half of the exponentials measured the same
 // time within 2 %: these loops are bound by latency, not by the special function unit.)
-template <bool FAR, int UN, typename T, typename F>
-__device__ __forceinline__ float row_weights(uint32_t taddr, uint32_t paddr, float c, float ref, F before_store) {
+template <bool FAR, int UN, typename T, typename F, typename G>
+__device__ __forceinline__ float row_weights(uint32_t taddr, uint32_t paddr, float c, float ref, F before_store,
+                                             G all_read) {
   uint32_t r[2][32];
   const float nref = -ref * c;
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -191,6 +193,7 @@ __device__ __forceinline__ float row_weights(uint32_t taddr, uint32_t paddr, flo
       uint32_t(&x)[32] = r[h];
       tmem_wait_ld();
       if (q < 3) FTM_TMEM_LD32_NOWAIT(taddr + (q + 1) * 32, r[h ^ 1]);
+      else all_read();
       uint32_t pk[16];
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
@@ -237,7 +240,8 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   uint64_t* m_full = drain + 1;     // 2: key bits of a tile, written by the TMA warp
   uint64_t* m_empty = drain + 3;    // 2: read by the softmax warps and the MMA warp
   uint64_t* pv_done = drain + 5;    // O and P of a tile free again (own P columns only)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 6);
+  uint64_t* s_empty = drain + 6;    // a tile's scores are all read (own P columns only)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 7);
 
   const int warp = uniform<E>(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -252,6 +256,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     mbar_init(b_full, 1);
     mbar_init(b_empty, 4);
     mbar_init(s_full, 1);
+    mbar_init(s_empty, 4);
     mbar_init(p_ready, 4);
     mbar_init(o_full, 1);
     mbar_init(drain, 1);
@@ -389,9 +394,14 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       more = walk.next(a, next);
       for (int j = 0; ok && j < n; ++j) {
         // P V of tile j and the scores of tile j + 1. Where P lies over S the scores come
-        // second (the tensor pipe runs in order), else first: the softmax waits for them.
+        // second (the tensor pipe runs in order), else as soon as tile j's have been read.
         const int kj = kn + j, s = kj % NS;
         const int kt = it.kt0 + j;
+        if (C::kOwnP && j + 1 < n) {
+          ok = arrived(j + 1) && mbar_wait_warp(s_empty, kj & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 6));
+          if (!ok) break;
+          scores(j + 1);
+        }
         ok = mbar_wait_warp(&v_full[s], (kj / NS) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 2));
         if (ok && a.key_mask)
           ok = mbar_wait_warp(&m_full[kj & 1], (kj >> 1) & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 5));
@@ -412,9 +422,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           fence_proxy_async_smem();
           __syncwarp();
         }
-        if (C::kOwnP && j + 1 < n) ok = arrived(j + 1);
-        ok = ok && mbar_wait_warp(p_ready, kj & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 3));
-        if (ok && C::kOwnP && j + 1 < n) scores(j + 1);
+        ok = mbar_wait_warp(p_ready, kj & 1, a.err, err_code(KERNEL_ATTN, ROLE_MMA, 3));
         if (!ok) break;
         tc_fence_after();
         {
@@ -459,7 +467,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         reinterpret_cast<uint4*>(out)[i < lo * per ? i : hi * per + (i - lo * per)] = make_uint4(0, 0, 0, 0);
     }
     bool ok = true;
-    while (ok && walk.next(a, it)) {
+    for (bool more = walk.next(a, it); ok && more;) {
       const bool live = tok < it.nq && row < a.group * a.tq;
       const int seen = a.causal ? min(it.klen, it.pos0 + tok + it.off + 1) : it.klen;
       float m = -INFINITY, l = 0.f;
@@ -525,8 +533,14 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         // c t - c ref in one rounding, unless a bias has put the whole row far from 0 (down to
         // the type's lowest value, used as a mask): then the difference first, which is exact
         const bool far = BIAS && __any_sync(0xffffffffu, fabsf(ref) > 1024.f);
-        if (far) l += row_weights<true, 1, T>(lanes, lanes + C::kColP, c, ref, pv_wait);
-        else l += row_weights<false, C::kUnroll, T>(lanes, lanes + C::kColP, c, ref, pv_wait);
+        auto all_read = [&] {
+          if (!C::kOwnP) return;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_empty);
+        };
+        if (far) l += row_weights<true, 1, T>(lanes, lanes + C::kColP, c, ref, pv_wait, all_read);
+        else l += row_weights<false, C::kUnroll, T>(lanes, lanes + C::kColP, c, ref, pv_wait, all_read);
         if (!ok) break;
         tmem_wait_st();
         tc_fence_before();
@@ -535,14 +549,15 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       }
       if (!ok) break;
       const bool any = it.kt1 > it.kt0;
+      const int slot = it.slot;
+      const size_t orow = (static_cast<size_t>(it.q0) + tok) * a.heads + it.head * a.group + gi;
+      more = walk.next(a, it);     // (some hundred clocks of divisions: under the last P V)
       if (any) {
         ok = mbar_wait_warp(o_full, on & 1, a.err, err_code(KERNEL_ATTN, ROLE_EPILOGUE, 3));
         if (!ok) break;
         ++on;
         tc_fence_after();
       }
-      const int head = it.head * a.group + gi;
-      const size_t orow = (static_cast<size_t>(it.q0) + tok) * a.heads + head;
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll 1
       for (int q = 0; q * 32 < a.dim; ++q) {
@@ -555,8 +570,8 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           for (int e = 0; e < 32; ++e) o[e] = 0;
         }
         if (!live) continue;
-        if (it.slot >= 0) {
-          float* po = a.part_o + (static_cast<size_t>(it.slot) * a.group + gi) * DP + q * 32;
+        if (slot >= 0) {
+          float* po = a.part_o + (static_cast<size_t>(slot) * a.group + gi) * DP + q * 32;
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             reinterpret_cast<uint4*>(po)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
@@ -573,7 +588,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           }
         }
       }
-      if (live && it.slot >= 0) a.part_ml[static_cast<size_t>(it.slot) * a.group + gi] = make_float2(m, l);
+      if (live && slot >= 0) a.part_ml[static_cast<size_t>(slot) * a.group + gi] = make_float2(m, l);
       if (live && a.stats)   // a row without keys: p = 2^-inf = 0 in the backward
         a.stats[orow] = l > 0.f || l != l ? make_float2(m, __log2f(l)) : make_float2(0.f, INFINITY);
       tc_fence_before();   // O read before the next item's first P V is released by p_ready
