@@ -89,7 +89,7 @@ class Attention(ctypes.Structure):
                 ("v", _vp), ("v_row_stride", _i64), ("v_head_stride", _i64), ("v_batch_stride", _i64),
                 ("key_mask", _vp), ("bias", _vp), ("bias_seqs", _i32),
                 ("bias_row_stride", _i64), ("bias_head_stride", _i64), ("bias_batch_stride", _i64),
-                ("out", _vp), ("stats", _vp)]
+                ("out", _vp), ("stats", _vp), ("out_low", _vp)]
 
 
 _PP = ctypes.POINTER(Problem)

@@ -582,9 +582,16 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             float f[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(o[e * 8 + k]) * inv;
-            *reinterpret_cast<uint4*>(out + orow * a.dim + q * 32 + e * 8) =
-                make_uint4(pack16<T>(f[0], f[1]), pack16<T>(f[2], f[3]), pack16<T>(f[4], f[5]),
-                           pack16<T>(f[6], f[7]));
+            uint32_t w[4], low[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              w[k] = pack16<T>(f[2 * k], f[2 * k + 1]);
+              const float2 r = unpack2<T>(w[k]);
+              low[k] = pack16<T>(f[2 * k] - r.x, f[2 * k + 1] - r.y);
+            }
+            const size_t at = orow * a.dim + q * 32 + e * 8;
+            *reinterpret_cast<uint4*>(out + at) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (a.out_low) *reinterpret_cast<uint4*>(static_cast<T*>(a.out_low) + at) = make_uint4(low[0], low[1], low[2], low[3]);
           }
         }
       }

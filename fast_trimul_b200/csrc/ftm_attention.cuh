@@ -43,6 +43,7 @@ struct AttnArgs {
   const void* o;             // forward output (backward)
   const void* g;             // its gradient: strides in elements
   long long g_row, g_head;
+  void* out_low;             // what rounding left of the output, for the backward; or null
   float2* stats;             // (row maximum m, log2 of the row sum) per (row, head)
   float4* bstats;            // backward: (see attn_delta_kernel)
   float* part_o;             // cache walk: partial results of split sequences

@@ -36,7 +36,7 @@ int check(const ftm_attention* p) {
       (k_tiles + p->sequences) * p->kv_heads * (p->kv_lengths ? p->sequences : 1) > kMaxRows)
     return FTM_BAD_SHAPE;
   if (p->kv_lengths) {
-    if (p->cu_q || p->cu_k || p->key_mask || p->bias || p->causal || p->stats) return FTM_BAD_ARGUMENT;
+    if (p->cu_q || p->cu_k || p->key_mask || p->bias || p->causal || p->stats || p->out_low) return FTM_BAD_ARGUMENT;
     if (p->q_len != 1 || p->q_rows != p->sequences) return FTM_BAD_SHAPE;
     if (!stride_ok(p->k_batch_stride, p->sequences) || !stride_ok(p->v_batch_stride, p->sequences))
       return FTM_BAD_ALIGN;
@@ -55,7 +55,7 @@ int check(const ftm_attention* p) {
       return FTM_BAD_ALIGN;
   }
   if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->v, 16) || !aligned(p->out, 16) ||
-      !aligned(p->stats, 8) || !stride_ok(p->q_row_stride, p->q_rows) ||
+      !aligned(p->stats, 8) || !aligned(p->out_low, 16) || !stride_ok(p->q_row_stride, p->q_rows) ||
       !stride_ok(p->q_head_stride, p->heads) || !stride_ok(p->k_row_stride, p->kv_rows) ||
       !stride_ok(p->k_head_stride, p->kv_heads) || !stride_ok(p->v_row_stride, p->kv_rows) ||
       !stride_ok(p->v_head_stride, p->kv_heads))
@@ -198,6 +198,7 @@ bool fill(AttnLaunch& l, const ftm_attention* p, int dev, int* err, int* host_er
   a.splits = a.kv_splits = 1;
   a.out = p->out;
   a.stats = reinterpret_cast<float2*>(p->stats);
+  a.out_low = p->out_low;
   a.err = err;
   a.host_err = host_err;
   const char* stall = getenv("FTM_TEST_STALL");

@@ -55,12 +55,14 @@ attn_delta_kernel(const __grid_constant__ AttnArgs a, int lanes, int bias) {
     if (i < n && l * 8 < a.dim) {
       const long long row = i / a.heads;
       const int head = static_cast<int>(i - row * a.heads);
-      float x[8], y[8];
+      float x[8], y[8], z[8] = {};
+      if (a.out_low)
+        unpack8(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.out_low) + i * a.dim + l * 8), IsBf16<T>::v, z);
       unpack8(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.o) + i * a.dim + l * 8), IsBf16<T>::v, x);
       unpack8(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.g) + row * a.g_row + head * a.g_head + l * 8),
               IsBf16<T>::v, y);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s = fmaf(x[k], y[k], s);
+      for (int k = 0; k < 8; ++k) s = fmaf(x[k] + z[k], y[k], s);
     }
     for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (i < n && l == 0) {

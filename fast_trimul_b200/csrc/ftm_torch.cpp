@@ -239,7 +239,7 @@ Tensor made_ready(const Tensor& t) {
 }
 
 ftm_attention problem(const Call& c, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bias,
-                      const Tensor& out, const Tensor& stats) {
+                      const Tensor& out, const Tensor& stats, const Tensor& low) {
   const bool batched = k.dim() == 4;
   const int64_t kr = k.dim() - 3;
   ftm_attention p{};
@@ -278,6 +278,7 @@ ftm_attention problem(const Call& c, const Tensor& q, const Tensor& k, const Ten
   }
   p.out = out.data_ptr();
   p.stats = stats.defined() ? stats.data_ptr<float>() : nullptr;
+  p.out_low = ptr(low);
   return p;
 }
 
@@ -285,19 +286,27 @@ Tensor bytes_on(const Tensor& like, size_t n) {
   return n ? at::empty({static_cast<int64_t>(n)}, like.options().dtype(at::kByte)) : Tensor();
 }
 
-Tensor attend(const Call& c, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bias, Tensor* stats,
-              Tensor* lists) {
+// what a backward needs of the forward beside its output
+struct Kept {
+  Tensor stats, low, lists;
+};
+
+Tensor attend(const Call& c, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bias, Kept* kept) {
   const c10::cuda::OptionalCUDAGuard guard(q.device());
-  const int train = stats != nullptr;
+  const int train = kept != nullptr;
+  Kept none;
+  Kept& t = train ? *kept : none;
   Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
-  if (train) *stats = at::empty({q.size(0), q.size(1), 2}, q.options().dtype(at::kFloat));
-  const ftm_attention p = problem(c, q, k, v, bias, out, train ? *stats : Tensor());
+  if (train) {
+    t.stats = at::empty({q.size(0), q.size(1), 2}, q.options().dtype(at::kFloat));
+    t.low = at::empty_like(out);
+  }
+  const ftm_attention p = problem(c, q, k, v, bias, out, t.stats, t.low);
   const size_t n = lib.at_bytes(&p, train);
-  Tensor ws = bytes_on(q, n);
+  t.lists = bytes_on(q, n);
   const Words& w = words[q.get_device()];
-  check(lib.at_fwd(&p, train, ptr(ws), n, w.dev, const_cast<int*>(w.host), stream_of(q)), "ftm_attention_fwd");
+  check(lib.at_fwd(&p, train, ptr(t.lists), n, w.dev, const_cast<int*>(w.host), stream_of(q)), "ftm_attention_fwd");
   count(true);
-  if (lists) *lists = ws;
   return out;
 }
 
@@ -305,9 +314,9 @@ struct Attention : torch::autograd::Function<Attention> {
   // `ready_bias` (what the kernels read) rides in the call: only `bias` itself has a gradient
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias,
                         const Call& c) {
-    Tensor stats, lists;
-    Tensor out = attend(c, q, k, v, c.ready_bias, &stats, &lists);
-    ctx->save_for_backward({q, k, v, c.ready_bias, out, stats, lists, c.cu_q, c.cu_k, c.mask});
+    Kept t;
+    Tensor out = attend(c, q, k, v, c.ready_bias, &t);
+    ctx->save_for_backward({q, k, v, c.ready_bias, out, t.stats, t.lists, c.cu_q, c.cu_k, c.mask, t.low});
     ctx->saved_data["n"] = std::vector<int64_t>{c.seqs, c.q_len, c.kv_len, c.bias_seqs, c.causal};
     ctx->saved_data["scale"] = c.scale;
     ctx->saved_data["held"] = c.held;
@@ -357,7 +366,7 @@ struct Attention : torch::autograd::Function<Attention> {
     if (bias.defined() && ctx->needs_input_grad(3))
       db = at::empty(ctx->saved_data["bias"].toIntVector(), q.options().memory_format(at::MemoryFormat::Contiguous));
     if (!dq.defined() && !dk.defined() && !db.defined()) return res;
-    const ftm_attention p = problem(c, q, k, v, bias, out, stats);
+    const ftm_attention p = problem(c, q, k, v, bias, out, stats, s[10]);
     const size_t bytes = lib.at_bwd_bytes(&p, db.defined());
     Tensor ws = bytes_on(q, bytes);
     const Words& w = words[q.get_device()];
@@ -379,7 +388,7 @@ Tensor run(const Call& c, const Tensor& q, const Tensor& k, const Tensor& v, con
                                      (has(bias) && bias->requires_grad())))
     return Attention::apply(q, k, v, bias, c);
   const at::AutoDispatchBelowAutograd below;
-  return attend(c, q, k, v, c.ready_bias, nullptr, nullptr);
+  return attend(c, q, k, v, c.ready_bias, nullptr);
 }
 
 // q, k, v of one 16-bit type on one GPU whose error words are known and clear, heads that
@@ -437,7 +446,7 @@ py::object cached(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   c.scale = s;
   c.lengths = lengths;
   const at::AutoDispatchBelowAutograd below;
-  return py::cast(attend(c, q, k, v, Tensor(), nullptr, nullptr));
+  return py::cast(attend(c, q, k, v, Tensor(), nullptr));
 }
 
 py::object pair(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias, const OptTensor& mask,

@@ -385,6 +385,9 @@ typedef struct {
   int64_t bias_row_stride, bias_head_stride, bias_batch_stride;
   void* out;
   float* stats; /* forward: NULL if no backward follows; 2 * q_rows * heads floats */
+  void* out_low; /* with stats, or NULL: like out, what its rounding left of the result. The backward
+                    forms rowsum(grad * out) of both: of out alone, dq and dk are off by up to a
+                    tenth more */
 } ftm_attention;
 /* Scratch of a forward (0: none needed, or bad arguments). With `train`, a packed call also
  * leaves there what its backward reads. err_word: a zeroed device word, as in the stages;

@@ -1,5 +1,7 @@
 """The attention kernels against 64 bits, with bounds derived in attention_reference.py."""
 
+import math
+
 import pytest
 import torch
 
@@ -231,6 +233,25 @@ def test_gradients_against_differences():
     mine = sum((a.double() * d).sum() for a, d in zip(grads, dirs)).item()
     size = sum((a.double() * d).abs().sum() for a, d in zip(grads, dirs)).item()
     assert abs(slope - mine) < 2 * 2 ** -11 * size      # each term is off by a few half steps at most
+
+
+@pytest.mark.parametrize("n, d, dtype", [(128, 64, torch.float16), (400, 32, BF), (96, 128, BF)])
+def test_gradients_lose_no_more_than_two_roundings(n, d, dtype):
+    # dS and the result are each rounded once, independently and by the same relative size, so
+    # the error's norm is sqrt(2) = 1.41 times the result's rounding alone; 1.5 leaves 6 % for the
+    # spread over a few thousand elements. (rowsum(grad * out) of the rounded output gave 1.55.)
+    from fast_trimul_b200.functional import packed_attention
+    q, k, v = (t.detach().requires_grad_() for t in qkv(n, n, 4, 4, d, dtype))
+    g = gen(9)(n, 4, d).to(dtype)
+    got = torch.autograd.grad(packed_attention(q, k, v, ends([n])), (q, k), g)
+    x = [t.detach().double().transpose(0, 1).requires_grad_() for t in (q, k, v)]
+    s = (x[0] @ x[1].transpose(1, 2)) * d ** -0.5
+    s = s.masked_fill(~torch.ones(n, n, dtype=torch.bool, device="cuda").tril(), -math.inf)
+    want = torch.autograd.grad(s.softmax(-1) @ x[2], x[:2], g.double().transpose(0, 1))
+    check_waits()
+    for a, b in zip(got, want):
+        b = b.transpose(0, 1)
+        assert (a.double() - b).norm() <= 1.5 * (b.to(dtype).double() - b).norm()
 
 
 def test_only_the_gradients_that_are_asked_for():
