@@ -310,7 +310,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         const int s = kn % NS;
         const uint32_t ph = ((kn / NS) & 1) ^ 1;
         ok = mbar_wait_warp(&k_empty[s], ph, a.err, err_code(KERNEL_ATTN, ROLE_PRODUCER, 2)) &&
-             !(a.test_stall && kn == 0);   // (then every wait of the block expires)
+             !(a.test_stall == STALL_FWD && kn == 0);   // (then every wait of the block expires)
         if (!ok) break;
         if (lane == 0) {
           mbar_arrive_expect_tx(&k_full[s], C::kTile);

@@ -55,7 +55,7 @@ struct AttnArgs {
   float* dbias_part;
   int* err;                  // device error word the waits poll
   int* host_err;             // pinned host word that learns of an expired wait; may be null
-  int test_stall;            // withhold the first K tile (failure tests)
+  int test_stall;            // withhold a tile (failure tests): STALL_*
 };
 
 // a role that gave up tells the host: polling a host word in the waits themselves would cross
@@ -168,6 +168,23 @@ __device__ __forceinline__ bool walk_item(const AttnArgs& a, int n, Item& it) {
     return true;
   }
   return walk_item_whole<KV>(a, n, it);
+}
+
+enum : int { STALL_FWD = 1, STALL_DQ = 2, STALL_DKV = 3 };
+
+// Named barrier that also tells whether `ok` holds in all of its threads: the warps that meet there
+// go on together or leave together, so none waits for one that gave up on an expired wait.
+__device__ __forceinline__ bool named_barrier_all(int id, int nthreads, bool ok) {
+  int all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.s32 p, %3, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, %2, p;\n\t"
+      "selp.s32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(id), "r"(nthreads), "r"(ok ? 1 : 0)
+      : "memory");
+  return all != 0;
 }
 
 // ------------------------------------------------------------------- tcgen05 forms

@@ -202,7 +202,11 @@ bool fill(AttnLaunch& l, const ftm_attention* p, int dev, int* err, int* host_er
   a.err = err;
   a.host_err = host_err;
   const char* stall = getenv("FTM_TEST_STALL");
-  a.test_stall = stall && strcmp(stall, "attention") == 0;
+  a.test_stall = !stall ? 0
+                 : strcmp(stall, "attention") == 0     ? STALL_FWD
+                 : strcmp(stall, "attention_dq") == 0  ? STALL_DQ
+                 : strcmp(stall, "attention_dkv") == 0 ? STALL_DKV
+                                                       : 0;
   return q_map(&l.m.q, p, p->q, p->q_row_stride, p->q_head_stride) &&
          kv_map(&l.m.k, p, p->k, p->k_row_stride, p->k_head_stride, p->k_batch_stride) &&
          kv_map(&l.m.v, p, p->v, p->v_row_stride, p->v_head_stride, p->v_batch_stride) &&

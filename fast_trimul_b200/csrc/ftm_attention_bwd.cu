@@ -219,7 +219,8 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
         }
         for (int t = it.kt0; ok && t < it.kt1; ++t) {
           const int s = kn % C::kK, sv = kn % C::kV;
-          ok = mbar_wait(&k_empty[s], ((kn / C::kK) & 1) ^ 1, a.err, err_code(KERNEL_DQ, ROLE_PRODUCER, 2));
+          ok = mbar_wait(&k_empty[s], ((kn / C::kK) & 1) ^ 1, a.err, err_code(KERNEL_DQ, ROLE_PRODUCER, 2)) &&
+               !(a.test_stall == STALL_DQ && blockIdx.x == 0 && kn == 0);
           if (!ok) break;
           mbar_arrive_expect_tx(&k_full[s], C::kTile);
           load_tile4<DP>(&maps.k, &k_full[s], sK + s * C::kTile, it.head, it.k0 + t * kTileRows, it.kb);
@@ -334,7 +335,8 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       zero_outside(a.cu_q, a.seqs, a.q_rows, static_cast<long long>(a.heads) * a.dim / 8, dq, threadIdx.x, kElemWarps * 32);
     int kn = 0, qn = 0;
     bool ok = true;
-    for (; ok && walk_item<false>(a, n, it); n += gridDim.x) {
+    // A failed wait is carried to the next barrier, where the quarter's warps leave together.
+    for (; walk_item<false>(a, n, it); n += gridDim.x) {
       const bool live = tok < it.nq && row < a.group * a.tq;
       const size_t orow = (static_cast<size_t>(it.q0) + tok) * a.heads + it.head * a.group + gi;
       const int seen = a.causal ? min(it.klen, it.pos0 + tok + it.off + 1) : it.klen;
@@ -346,9 +348,8 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
         const uint32_t on = (a.key_mask ? key_word(a, it, kt, part, lane) : 0xffffffffu) &
                             bits_below(seen - kt * kTileRows, part);
         const bool cut = __any_sync(0xffffffffu, on != 0xffffffffu);
-        ok = mbar_wait_warp(&s_full[b], (kn >> 1) & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 1));
+        ok = ok && mbar_wait_warp(&s_full[b], (kn >> 1) & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 1));
         if (BIAS) ok = ok && mbar_wait_warp(b_full, kn & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 2));
-        if (!ok) break;
         tc_fence_after();
         const uint32_t scol = lanes + (b ? 384 : 0);
         uint32_t r[32];
@@ -369,8 +370,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
           for (int e = 0; e < 32; ++e)
             if (!(on & (1u << e))) r[e] = 0u;
         }
-        ok = mbar_wait_warp(dp_full, kn & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 3));
-        if (!ok) break;
+        ok = ok && mbar_wait_warp(dp_full, kn & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 3));
         tc_fence_after();
         uint32_t pk[16], d[32];
         FTM_TMEM_LD32_NOWAIT(lanes + 128 + part * 32, d);
@@ -385,22 +385,22 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
           }
           pk[e / 2] = pack16<T>(x0, x1);
         }
-        named_barrier_sync(1 + quad, 128);   // the whole row of S has been read: dS goes over it
+        ok = named_barrier_all(1 + quad, 128, ok);   // the whole row of S has been read: dS goes over it
+        if (!ok) break;
         tmem_st16(scol + part * 16, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(ds_ready);
       }
-      if (!ok) break;
       const bool any = it.kt1 > it.kt0;
       if (any) {
-        ok = mbar_wait_warp(acc_full, qn & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 4));
         if (!ok) break;
+        ok = mbar_wait_warp(acc_full, qn & 1, a.err, err_code(KERNEL_DQ, ROLE_EPILOGUE, 4));
         ++qn;
         tc_fence_after();
       }
-      store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, a.scale, live, any, dq + orow * a.dim);
+      store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, a.scale, live && ok, any, dq + orow * a.dim);
       tc_fence_before();
     }
   }
@@ -508,7 +508,8 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       for (int t = it.kt0; t < it.kt1; ++t) {
         const int s = qn & 1;
         const uint32_t ph = ((qn >> 1) & 1) ^ 1;
-        ok = mbar_wait_warp(&q_empty[s], ph, a.err, err_code(KERNEL_DKV, ROLE_PRODUCER, 2)) &&
+        ok = !(a.test_stall == STALL_DKV && blockIdx.x == 0 && qn == 0) &&
+             mbar_wait_warp(&q_empty[s], ph, a.err, err_code(KERNEL_DKV, ROLE_PRODUCER, 2)) &&
              mbar_wait_warp(&g_empty[s], ph, a.err, err_code(KERNEL_DKV, ROLE_PRODUCER, 3)) &&
              (!BIAS || mbar_wait_warp(b_empty, (qn & 1) ^ 1, a.err, err_code(KERNEL_DKV, ROLE_PRODUCER, 4)));
         if (!ok) break;
@@ -654,7 +655,8 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     }
     int qn = 0, in = 0;
     bool ok = true;
-    for (; ok && walk_item<true>(a, n, it); n += gridDim.x) {
+    // A failed wait is carried to the next barrier, where the quarter's warps leave together.
+    for (; walk_item<true>(a, n, it); n += gridDim.x) {
       const int key = it.tile * kTileRows + row;
       const bool live = key < it.klen;
       const size_t orow = (static_cast<size_t>(it.k0) + key) * a.kv_heads + it.head;
@@ -667,10 +669,9 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         const int lo = a.causal ? max(0, min(kTileRows, (key - it.off - t * a.tq) * a.group)) : 0;
         const bool cut = gone || __any_sync(0xffffffffu, lo > 0);
         const float* col = sC + cb * 384;
-        ok = mbar_wait_warp(&c_full[cb], (qn / C::kCols) & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 1));
+        ok = ok && mbar_wait_warp(&c_full[cb], (qn / C::kCols) & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 1));
         if (BIAS) ok = ok && mbar_wait_warp(b_full, qn & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 2));
         ok = ok && mbar_wait_warp(s_full, qn & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 3));
-        if (!ok) break;
         tc_fence_after();
         uint32_t r[32];
         FTM_TMEM_LD32_NOWAIT(lanes + part * 32, r);
@@ -710,14 +711,14 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         uint32_t pk[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) pk[e / 2] = pack16<T>(__uint_as_float(r[e]), __uint_as_float(r[e + 1]));
-        named_barrier_sync(1 + quad, 128);   // the whole row of S^T has been read: P^T goes over it
+        ok = named_barrier_all(1 + quad, 128, ok);   // the whole row of S^T has been read: P^T goes over it
+        if (!ok) break;
         tmem_st16(lanes + part * 16, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready);
         ok = mbar_wait_warp(dp_full, qn & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 4));
-        if (!ok) break;
         tc_fence_after();
         uint32_t d[32];
         FTM_TMEM_LD32_NOWAIT(lanes + 128 + part * 32, d);
@@ -737,29 +738,29 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&c_empty[cb]);
-        named_barrier_sync(1 + quad, 128);
+        ok = named_barrier_all(1 + quad, 128, ok);
+        if (!ok) break;
         tmem_st16(lanes + 128 + part * 16, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(ds_ready);
       }
-      if (!ok) break;
       const bool any = it.kt1 > it.kt0;
       if (any) {
-        ok = mbar_wait_warp(acc_full, in & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 5));
         if (!ok) break;
+        ok = mbar_wait_warp(acc_full, in & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 5));
         ++in;
         tc_fence_after();
       }
       if (a.kv_splits > 1) {
         const size_t all = static_cast<size_t>(a.kv_rows) * a.kv_heads * a.dim;
         float* to = a.dkv_part + 2 * it.slot * all + orow * a.dim;
-        store_part<DP / 4>(lanes + 384, part * (DP / 4), a.dim, a.scale, live, any, to);
-        store_part<DP / 4>(lanes + 256, part * (DP / 4), a.dim, 1.f, live, any, to + all);
+        store_part<DP / 4>(lanes + 384, part * (DP / 4), a.dim, a.scale, live && ok, any, to);
+        store_part<DP / 4>(lanes + 256, part * (DP / 4), a.dim, 1.f, live && ok, any, to + all);
       } else {
-        store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, 1.f, live, any, dv + orow * a.dim);
-        store_acc<DP / 4>(lanes + 384, part * (DP / 4), a.dim, a.scale, live, any, dk + orow * a.dim);
+        store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, 1.f, live && ok, any, dv + orow * a.dim);
+        store_acc<DP / 4>(lanes + 384, part * (DP / 4), a.dim, a.scale, live && ok, any, dk + orow * a.dim);
       }
       tc_fence_before();
     }

@@ -653,6 +653,29 @@ def test_a_withheld_tile_is_reported_and_the_next_call_is_right(monkeypatch):
     check_waits()
 
 
+@pytest.mark.parametrize("kernel", ["dq", "dkv"])
+@pytest.mark.parametrize("bias", [False, True])
+def test_a_withheld_tile_of_a_backward_is_reported(monkeypatch, kernel, bias):
+    """One block's first tile is withheld while the others work: its waits expire, its warps leave
+    together, and the others see the error at a wait of theirs, whichever that is."""
+    from fast_trimul_b200 import _lib
+    from fast_trimul_b200.functional import pair_attention
+    x = [t.detach().requires_grad_() for t in pair_inputs(1, 60, 200, 4, 32, BF)]
+    if not bias:
+        x = x[:3] + [None]
+    g = gen(2)(1, 60, 200, 4, 32).to(BF)
+    grads = lambda: torch.autograd.grad(pair_attention(*x), [t for t in x if t is not None], g)   # noqa: E731
+    want = grads()
+    monkeypatch.setenv("FTM_TEST_STALL", "attention_" + kernel)
+    grads()
+    monkeypatch.delenv("FTM_TEST_STALL")
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.NativeKernelError):
+        grads()
+    assert all(torch.equal(a, b) for a, b in zip(grads(), want))
+    check_waits()
+
+
 # ----------------------------------------------------------------- the operators together
 def test_attention_block_trains_like_the_formula():
     """Norm, projections, packed attention and residual together, as a model uses them, against
