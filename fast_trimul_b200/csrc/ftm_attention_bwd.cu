@@ -24,8 +24,11 @@
 // block per SM: dq holds S twice (the next tile's scores are formed under this one's
 // elementwise part), dkv holds S^T, dP^T, dV, dK.
 //
-// A sequence of 8192 tokens, causal, 16 heads on 4, dim 128, bf16: dq 441 us, dkv 652 to 665 us
-// (935 and 830 TFLOP/s over the products they form; one large product reaches 1700).
+// A sequence of 8192 tokens, causal, 16 heads on 4, dim 128, bf16: dq 440 us, dkv 694 us
+// (935 and 790 TFLOP/s over the products they form; one large product reaches 1700). 20 us of
+// dkv's are the barriers that vote on expired waits; two buffers for the next item's Q and g, or
+// K and V, and finding that item under the last product gave 3 us of 331 at N = 250 and cost as
+// much at dim 128, so they are not there.
 #include <climits>
 
 #include "ftm_attention.cuh"

@@ -581,6 +581,17 @@ def test_nothing_to_attend_to_gives_zeros_whatever_the_inputs_hold():
         assert torch.equal(grad, torch.zeros_like(bad))
 
 
+def test_the_first_call_of_a_gpu_is_not_captured():
+    # its error word would be zeroed by the graph's replay alone
+    from fast_trimul_b200 import _lib
+    from fast_trimul_b200.ops.attention import AttentionErrorWord
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(8, device="cuda")
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(_lib.NativeDeclined):
+            AttentionErrorWord(torch.device("cuda", 0))
+
+
 @pytest.mark.parametrize("kind", ["packed", "pair", "layer_norm"])
 def test_second_derivatives_are_refused(kind):
     # a gradient taken with create_graph is right, and differentiating it raises
