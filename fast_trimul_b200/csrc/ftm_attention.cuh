@@ -55,6 +55,7 @@ struct AttnArgs {
   float* dbias_part;
   int* err;                  // device error word the waits poll
   int* host_err;             // pinned host word that learns of an expired wait; may be null
+  bool dbias_direct;         // the dq kernel writes dbias: one row per bias, all tiles met
   int test_stall;            // withhold a tile (failure tests): STALL_*
 };
 

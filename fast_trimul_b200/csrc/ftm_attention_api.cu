@@ -328,6 +328,8 @@ int ftm_attention_bwd(const ftm_attention* p, const void* grad, int64_t grad_row
   l.a.splits = w.splits;
   l.a.kv_splits = w.kv_splits;
   l.a.dkv_part = reinterpret_cast<float*>(ws + w.kv_part);
+  // (a causal walk leaves out the tiles whose bias' gradient is 0)
+  l.a.dbias_direct = dbias && dq && p->bias_seqs == 1 && l.dp == 64 && !p->causal;
   int launches = 1;
   if (launch_attn_delta(l) != cudaSuccess) return FTM_LAUNCH_FAILED;
   uint8_t* lists = static_cast<uint8_t*>(fwd_workspace);
@@ -351,7 +353,7 @@ int ftm_attention_bwd(const ftm_attention* p, const void* grad, int64_t grad_row
       ++launches;
     }
   }
-  if (dbias) {
+  if (dbias && !l.a.dbias_direct) {
     if (launch_attn_dbias(l) != cudaSuccess) return FTM_LAUNCH_FAILED;
     launches += w.splits > 1 ? 2 : 1;
   }

@@ -9,7 +9,8 @@
 //   dq     one query tile, loop over its key tiles:    S, dP -> dS;   dQ += dS K
 //   dkv    one key tile, loop over its query tiles:    S^T, dP^T -> P^T, dS^T;
 //          dV += P^T dO, dK += dS^T Q; with grouped heads the loop covers the whole group
-//   dbias  one tile of the bias, loop over the rows that share it, sums in registers
+//   dbias  one tile of the bias, loop over the rows that share it, sums in registers (a bias of
+//          one row alone: dq writes dS along)
 // Each result has one owner, so there are no atomics and a call gives the same bits every
 // time, at the price of forming S and dP twice (7 products instead of 5). fp32 everywhere
 // but the 16-bit operands P and dS, rounded once like the inputs of any product here.
@@ -150,6 +151,13 @@ __device__ __forceinline__ uint32_t key_word(const AttnArgs& a, const Item& it, 
 // --------------------------------------------------------------------------------- dq
 // K of a tile is held from its scores to dQ += dS K, two tiles of the loop: with two buffers the
 // next scores waited for their K to be loaded, 1800 clocks of a tile's 4400 at dim 128.
+// A bias that one row alone has (a single representation's attention) has dS itself for its
+// gradient, which the dq kernel then writes along: 2 x 1001 positions, 16 heads of 24, training
+// 180 us (dq 63) against 237 (dq 38, dbias 85) with the dbias kernel, which forms S and dP once
+// more. At DP = 128 shared memory has no room for the transposed tiles.
+template <int DP>
+constexpr bool kDirectBias = DP == 64;
+
 template <int DP, bool BIAS>
 struct DqCfg {
   static constexpr int kTile = DP / 64 * kBlk;
@@ -159,7 +167,8 @@ struct DqCfg {
   static constexpr int kOffV = kOffK + kK * kTile;
   static constexpr int kOffB = kOffV + kV * kTile;
   static constexpr int kOffBar = kOffB + (BIAS ? 2 * kBlk : 0);
-  static constexpr int kSmem = kOffBar + 256 + 1024;
+  static constexpr int kOffT = kOffBar + 256;      // a warp's 32 x 32 of dS, rows of 16 + 1 words
+  static constexpr int kSmem = kOffT + (kDirectBias<DP> && BIAS ? kElemWarps * 32 * 17 * 4 : 0) + 1024;
   static_assert(kSmem <= 232448, "dq exceeds 227 KB of shared memory");
 };
 
@@ -395,6 +404,24 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(ds_ready);
+        if (kDirectBias<DP> && BIAS && a.dbias_direct) {
+          // transposed in shared memory, so that a warp writes neighbours of one row at a time
+          uint32_t* tile = reinterpret_cast<uint32_t*>(smem + C::kOffT) + warp * 32 * 17;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) tile[lane * 17 + e] = pk[e];
+          __syncwarp();
+          const int col = kt * kTileRows + part * 32 + lane, row0 = it.pos0 + quad * 32;
+          if (col < a.k_len) {
+            uint16_t* to = static_cast<uint16_t*>(a.dbias) +
+                           ((static_cast<size_t>(it.seq) * a.heads + it.head) * a.q_len + row0) * a.k_len + col;
+            const int rows = min(32, a.q_len - row0);
+#pragma unroll 4
+            for (int y = 0; y < rows; ++y)
+              to[static_cast<size_t>(y) * a.k_len] =
+                  static_cast<uint16_t>(tile[y * 17 + (lane >> 1)] >> ((lane & 1) * 16));
+          }
+          __syncwarp();
+        }
       }
       const bool any = it.kt1 > it.kt0;
       if (any) {

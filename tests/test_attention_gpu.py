@@ -411,6 +411,29 @@ def pair_inputs(b, r, n, h, d, dtype, seed=0, biases=None):
     return q, k, v, x(biases or b, h, n, n).to(dtype)
 
 
+@pytest.mark.parametrize("n", [1, 2, 31, 33, 128, 129, 250, 301])
+@pytest.mark.parametrize("h,d,dtype", [(4, 24, BF), (2, 64, HF), (2, 96, BF)])
+def test_pair_a_bias_of_one_row_alone(n, h, d, dtype):
+    # its gradient is dS itself; masked keys, whatever they hold, and a row without any
+    q, k, v, bias = pair_inputs(2, 1, n, h, d, dtype, n)
+    mask = gen(n)(2, 1, n) > 0
+    mask[1] = False
+    bad = torch.where(mask[..., None, None], v, torch.full_like(v, float("nan")))
+    check_pair(q, k, v, bias)
+    got = check_pair(q, k, bad, bias, mask)
+    assert torch.equal(got[4][1], torch.zeros_like(got[4][1]))
+    # the bias' gradient alone (from another kernel: within a rounding), and all but it
+    from fast_trimul_b200.functional import pair_attention
+    b = bias.clone().requires_grad_()
+    g = gen(8)(*q.shape).to(dtype)
+    (alone,) = torch.autograd.grad(pair_attention(q, k, v, b), b, g)
+    all_of = train(pair_attention, (q, k, v, bias), g)
+    assert (alone.float() - all_of[4].float()).norm() <= 1e-2 * all_of[4].float().norm() + 1e-6
+    x = [t.clone().requires_grad_() for t in (q, k, v)]
+    for a, c in zip(torch.autograd.grad(pair_attention(*x, bias), x, g), all_of[1:4]):
+        assert torch.equal(a, c)
+
+
 @pytest.mark.parametrize("n", [1, 7, 8, 64, 127, 128, 129, 200])
 @pytest.mark.parametrize("h,d,dtype", [(4, 32, BF), (2, 64, HF), (3, 24, BF), (2, 128, BF)])
 def test_pair_lengths(n, h, d, dtype):
