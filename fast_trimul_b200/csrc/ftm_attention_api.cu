@@ -48,6 +48,7 @@ int check(const ftm_attention* p) {
       return FTM_BAD_SHAPE;
   }
   if (p->bias) {
+    if (p->causal) return FTM_BAD_ARGUMENT;     // its gradient's kernel knows key masks only
     if (p->heads != p->kv_heads || p->bias_seqs < 1 || p->sequences % p->bias_seqs) return FTM_BAD_SHAPE;
     if (!aligned(p->bias, 16) || !stride_ok(p->bias_row_stride, p->q_len) ||
         !stride_ok(p->bias_head_stride, p->heads) ||
@@ -328,8 +329,7 @@ int ftm_attention_bwd(const ftm_attention* p, const void* grad, int64_t grad_row
   l.a.splits = w.splits;
   l.a.kv_splits = w.kv_splits;
   l.a.dkv_part = reinterpret_cast<float*>(ws + w.kv_part);
-  // (a causal walk leaves out the tiles whose bias' gradient is 0)
-  l.a.dbias_direct = dbias && dq && p->bias_seqs == 1 && l.dp == 64 && !p->causal;
+  l.a.dbias_direct = dbias && dq && p->bias_seqs == 1 && l.dp == 64;
   int launches = 1;
   if (launch_attn_delta(l) != cudaSuccess) return FTM_LAUNCH_FAILED;
   uint8_t* lists = static_cast<uint8_t*>(fwd_workspace);

@@ -363,7 +363,7 @@ int ftm_layer_norm_bwd(const void* x, int32_t dtype, int64_t x_row_stride, const
  *            [0, kv_lengths[i]) of batch entry i, whose kv_rows rows are k_batch_stride apart.
  * With `causal`, query i of a sequence sees keys j <= i + (keys - queries): aligned to the
  * last key. key_mask (kv_rows bytes, may be NULL): keys with 0 are not seen, whatever K and V
- * hold there. bias (may be NULL; uniform only, heads == kv_heads, q_len x kv_len rows): one per
+ * hold there. bias (may be NULL; uniform and not causal, heads == kv_heads, q_len x kv_len rows): one per
  * run of bias_seqs consecutive sequences and head.
  * Strides are in elements, multiples of 8; pointers 16-byte aligned; the head dimension is
  * contiguous, a multiple of 8, at most 128. out is contiguous (q_rows, heads, head_dim). */

@@ -156,6 +156,19 @@ def test_c_entry_points_check_their_arguments_before_the_device():
     assert fwd(ws=None) == W and fwd(n=8) == W
 
 
+def test_a_bias_with_a_causal_call_is_refused():
+    p = 1 << 20
+    prob = _lib.Attention(dtype=_lib.BF16, heads=2, kv_heads=2, head_dim=64, causal=1, scale=0.125, sequences=2,
+                          q_len=50, kv_len=50, q_rows=100, kv_rows=100, q=p, q_row_stride=128, q_head_stride=64, k=p,
+                          k_row_stride=128, k_head_stride=64, v=p, v_row_stride=128, v_head_stride=64, bias=p,
+                          bias_seqs=1, bias_row_stride=56, bias_head_stride=2800, bias_batch_stride=5600, out=p)
+    assert _lib.load().ftm_attention_fwd(prob, 0, None, 0, p, None, None) == _lib.BAD_ARGUMENT
+    prob.causal = 0
+    assert _lib.load().ftm_attention_fwd(prob, 0, None, 0, None, None, None) == _lib.BAD_ARGUMENT   # no error word
+    prob.bias_row_stride = 50
+    assert _lib.load().ftm_attention_fwd(prob, 0, None, 0, p, None, None) == _lib.BAD_ALIGN
+
+
 def test_workspace_sizes():
     lib = _lib.load()
     assert lib.ftm_attention_workspace_bytes(None, 0) == 0

@@ -710,6 +710,62 @@ def test_a_withheld_tile_of_a_backward_is_reported(monkeypatch, kernel, bias):
     check_waits()
 
 
+@pytest.mark.parametrize("seqs, nq, nk, h, hk, d, causal, bias", [
+    (3, 50, 200, 4, 2, 64, 1, 0), (2, 200, 50, 6, 2, 128, 1, 0), (2, 129, 300, 4, 4, 32, 0, 1),
+    (4, 1, 130, 2, 2, 24, 0, 2), (2, 300, 129, 2, 2, 128, 0, 1), (6, 70, 90, 2, 2, 16, 0, 3)])
+def test_the_uniform_form_of_the_c_entries(seqs, nq, nk, h, hk, d, causal, bias):
+    """Sequences of one length with other numbers of keys than queries; `bias` rows share one."""
+    from fast_trimul_b200 import _lib
+    from fast_trimul_b200.ops.attention import attention_error_word
+    lib, e = _lib.load(), attention_error_word()
+    q, k, v = qkv(seqs * nq, seqs * nk, h, hk, d, BF, seqs)
+    q, k, v = (t.detach().contiguous() for t in (q, k, v))
+    g = gen(3)(seqs * nq, h, d).to(BF)
+    wide, n = (nk + 7) // 8 * 8, seqs // bias if bias else 0
+    b = gen(4)(n, h, nq, wide).to(BF) if bias else None
+    new = lambda *s: torch.full(s, float("nan"), dtype=BF, device="cuda")   # noqa: E731
+    out, low, dq, dk, dv = new(*q.shape), new(*q.shape), new(*q.shape), new(*k.shape), new(*k.shape)
+    db, st = new(n, h, nq, nk), torch.empty(seqs * nq, h, 2, device="cuda")
+    p = _lib.Attention(dtype=_lib.BF16, heads=h, kv_heads=hk, head_dim=d, causal=causal, scale=d ** -0.5,
+                       sequences=seqs, q_len=nq, kv_len=nk, q_rows=seqs * nq, kv_rows=seqs * nk, q=q.data_ptr(),
+                       q_row_stride=h * d, q_head_stride=d, k=k.data_ptr(), k_row_stride=hk * d, k_head_stride=d,
+                       v=v.data_ptr(), v_row_stride=hk * d, v_head_stride=d, out=out.data_ptr(), stats=st.data_ptr(),
+                       out_low=low.data_ptr())
+    if bias:
+        p.bias, p.bias_seqs, p.bias_row_stride = b.data_ptr(), bias, wide
+        p.bias_head_stride, p.bias_batch_stride = nq * wide, h * nq * wide
+    s = torch.cuda.current_stream().cuda_stream
+    assert lib.ftm_attention_workspace_bytes(p, 1) == 0
+    size = lib.ftm_attention_bwd_workspace_bytes(p, 1 if bias else 0)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    assert lib.ftm_attention_fwd(p, 1, None, 0, e.ptr, e.host_ptr, s) == _lib.OK
+    assert lib.ftm_attention_bwd(p, g.data_ptr(), h * d, d, None, 0, ws.data_ptr(), size, dq.data_ptr(), dk.data_ptr(),
+                                 dv.data_ptr(), db.data_ptr() if bias else None, e.ptr, e.host_ptr, s) == _lib.OK
+    check_waits()
+    w = ref.Sums(q, k, db if bias else None)
+    keep = torch.ones(nq, nk, dtype=torch.bool, device="cuda")
+    if causal:
+        keep = keep.tril(nk - nq)
+    x = [t.double() for t in (q, k, v, g)]
+    for i in range(seqs):
+        a, c = slice(i * nq, (i + 1) * nq), slice(i * nk, (i + 1) * nk)
+        for j in range(h):
+            jk = j // (h // hk)
+            m = b[i // bias, j, :, :nk].double() if bias else None
+            res, off = ref.head(x[0][a, j], x[1][c, jk], x[2][c, jk], x[3][a, j], d ** -0.5, keep, m, 2.0 ** -8)
+            w.o[a, j], w.dq[a, j], w.eo[a, j], w.edq[a, j] = res[0], res[1], off[0], off[1]
+            w.dk[c, jk] += res[2]
+            w.dv[c, jk] += res[3]
+            w.edk[c, jk] += off[2]
+            w.edv[c, jk] += off[3]
+            if bias:
+                w.db[i // bias, j] += res[4]
+                w.edb[i // bias, j] += off[4]
+    for name, got, want, off in (("o", out, w.o, w.eo), ("dq", dq, w.dq, w.edq), ("dk", dk, w.dk, w.edk),
+                                 ("dv", dv, w.dv, w.edv), *((("dbias", db, w.db, w.edb),) if bias else ())):
+        ref.close(got, want, off, name)
+
+
 # ----------------------------------------------------------------- the operators together
 def test_attention_block_trains_like_the_formula():
     """Norm, projections, packed attention and residual together, as a model uses them, against
