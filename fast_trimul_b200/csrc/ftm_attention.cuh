@@ -372,6 +372,14 @@ __device__ __forceinline__ void add_bias(uint32_t (&r)[32], const uint8_t* block
   }
 }
 
+// The kv walk, causal: columns of a query tile in front of the first query that sees a key. `ahead`:
+// tokens from the tile's first to that query. They are cut to a tile before they are multiplied:
+// tokens times the heads of a group may pass 32 bits (17e6 keys in front of one query of 128 heads).
+__host__ __device__ __forceinline__ int columns_before(int ahead, int group) {
+  const int t = ahead < 0 ? 0 : ahead < kTileRows ? ahead : kTileRows;
+  return t * group < kTileRows ? t * group : kTileRows;
+}
+
 // bits [0, lim) of a 128-bit row
 __device__ __forceinline__ uint32_t bits_below(int lim, int word) {
   const int n = lim - word * 32;

@@ -696,7 +696,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       for (int t = it.kt0; t < it.kt1; ++t, ++qn) {
         const int cb = qn % C::kCols;
         // queries in front of the first one that sees this key (causal): columns below `lo`
-        const int lo = a.causal ? max(0, min(kTileRows, (key - it.off - t * a.tq) * a.group)) : 0;
+        const int lo = a.causal ? columns_before(key - it.off - t * a.tq, a.group) : 0;
         const bool cut = gone || __any_sync(0xffffffffu, lo > 0);
         const float* col = sC + cb * 384;
         ok = ok && mbar_wait_warp(&c_full[cb], (qn / C::kCols) & 1, a.err, err_code(KERNEL_DKV, ROLE_EPILOGUE, 1));

@@ -1,0 +1,49 @@
+"""Limits of the attention kernels that need no GPU: their tile arithmetic near 32 bits, compiled for
+the host."""
+
+import os
+import shutil
+import subprocess
+
+import pytest
+
+from conftest import ROOT
+
+CSRC = os.path.join(ROOT, "fast_trimul_b200", "csrc")
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    """Calls a function of the kernels' header with whole numbers, on the host."""
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("needs nvcc")
+    at = tmp_path_factory.mktemp("host")
+
+    def build(name, args):
+        src, exe = at / f"{name}.cu", at / name
+        if not exe.exists():
+            values = ", ".join(f"std::atoi(argv[i + {i}])" for i in range(args))
+            src.write_text('#include <cstdio>\n#include <cstdlib>\n#include "ftm_attention.cuh"\n'
+                           "int main(int argc, char** argv) {\n"
+                           f"  for (int i = 1; i + {args - 1} < argc; i += {args})"
+                           f' std::printf("%d\\n", ftm::{name}({values}));\n' "}\n")
+            subprocess.run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "--expt-relaxed-constexpr",
+                            "-I", CSRC, "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)],
+                           check=True, capture_output=True)
+        return str(exe)
+
+    def call(name, rows):
+        exe = build(name, len(rows[0]))
+        out = subprocess.run([exe, *[str(x) for r in rows for x in r]], check=True, capture_output=True, text=True)
+        return [int(x) for x in out.stdout.split()]
+
+    return call
+
+
+FAR = [0, 1, 2, 63, 64, 127, 128, 129, 16_777_216, 16_777_217, 17_000_000, 33_554_432, 2 ** 30, 2 ** 31 - 1024]
+
+
+def test_columns_in_front_of_the_first_query(host):
+    rows = [(s * n, g) for n in FAR for s in (1, -1) for g in (1, 2, 3, 64, 127, 128)]
+    assert host("columns_before", rows) == [max(0, min(128, a * g)) for a, g in rows]
