@@ -380,6 +380,13 @@ __host__ __device__ __forceinline__ int columns_before(int ahead, int group) {
   return t * group < kTileRows ? t * group : kTileRows;
 }
 
+// Rows of a query tile that hold queries, where `left` tokens of the sequence remain from its first
+// token on; cut before they are multiplied, as above (a negative product would clear memory in front
+// of the tile).
+__host__ __device__ __forceinline__ int rows_held(int left, int tq, int group) {
+  return (left < tq ? left : tq) * group;
+}
+
 // bits [0, lim) of a 128-bit row
 __device__ __forceinline__ uint32_t bits_below(int lim, int word) {
   const int n = lim - word * 32;

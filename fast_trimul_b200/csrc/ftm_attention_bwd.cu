@@ -602,7 +602,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     auto arrived = [&](uint64_t* full, uint8_t* tiles, int i, int t, int site) -> bool {
       const int s = i & 1;
       if (!mbar_wait_warp(&full[s], (i >> 1) & 1, a.err, err_code(KERNEL_DKV, ROLE_MMA, site))) return false;
-      const int valid = (it.nq - t * a.tq) * a.group;
+      const int valid = rows_held(it.nq - t * a.tq, a.tq, a.group);
       if (valid < a.group * a.tq) {
         zero_rows_from<DP>(tiles + s * C::kTile, valid, lane);
         fence_proxy_async_smem();

@@ -47,3 +47,8 @@ FAR = [0, 1, 2, 63, 64, 127, 128, 129, 16_777_216, 16_777_217, 17_000_000, 33_55
 def test_columns_in_front_of_the_first_query(host):
     rows = [(s * n, g) for n in FAR for s in (1, -1) for g in (1, 2, 3, 64, 127, 128)]
     assert host("columns_before", rows) == [max(0, min(128, a * g)) for a, g in rows]
+
+
+def test_rows_of_a_query_tile(host):
+    rows = [(n, 128 // g, g) for n in FAR[1:] for g in (1, 2, 3, 64, 127, 128)]
+    assert host("rows_held", rows) == [min(n, tq) * g for n, tq, g in rows]
