@@ -43,6 +43,10 @@ struct AttnArgs {
   const void* o;             // forward output (backward)
   const void* g;             // its gradient: strides in elements
   long long g_row, g_head;
+  const void* v;             // (backward in fp16: its row norms)
+  long long v_row, v_head;
+  float2* norms;             // largest row norms (of g, of v), a pair per block of the delta kernel
+  int norm_parts;
   void* out_low;             // what rounding left of the output, for the backward; or null
   float2* stats;             // (row maximum m, log2 of the row sum) per (row, head)
   float4* bstats;            // backward: (see attn_delta_kernel)
@@ -414,6 +418,8 @@ cudaError_t launch_attn_lists(const AttnLaunch& l, int2* q_list, int q_cap, int2
                               int* counts);
 cudaError_t launch_pad_rows(const void* src, long long src_stride, void* dst, long long dst_stride, long long rows,
                             int cols, int sms, cudaStream_t stream);
+constexpr int kDeltaBlocks = 8;   // per SM, at most
+int attn_delta_grid(const AttnLaunch& l);
 cudaError_t launch_attn_delta(const AttnLaunch& l);
 cudaError_t launch_attn_dq(const AttnLaunch& l);
 cudaError_t launch_attn_dkv(const AttnLaunch& l);

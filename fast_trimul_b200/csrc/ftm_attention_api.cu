@@ -125,14 +125,15 @@ FwdSpace fwd_space(const ftm_attention* p, int train, int sms) {
   return w;
 }
 
-// backward: [row constants][parts of dk and dv][parts of the bias gradient]
+// backward: [row constants][row norms, fp16][parts of dk and dv][parts of the bias gradient]
 struct BwdSpace {
-  size_t kv_part, part, total;
+  size_t norms, kv_part, part, total;
   int splits, kv_splits;
 };
 BwdSpace bwd_space(const ftm_attention* p, int want_dbias, int sms) {
   BwdSpace w{};
-  w.kv_part = up256(size_t(p->q_rows) * p->heads * sizeof(float4));
+  w.norms = up256(size_t(p->q_rows) * p->heads * sizeof(float4));
+  w.kv_part = w.norms + (p->dtype == FTM_F16 ? up256(size_t(sms) * kDeltaBlocks * sizeof(float2)) : 0);
   w.part = w.kv_part;
   // Few key tiles (one key / value head, a few thousand keys) leave SMs idle: the query tiles of
   // each are split over up to 8 blocks, at least 4 tiles each, and the parts added up. One
@@ -320,7 +321,12 @@ int ftm_attention_bwd(const ftm_attention* p, const void* grad, int64_t grad_row
   l.a.g = grad;
   l.a.g_row = p->q_rows > 1 ? grad_row_stride : 0;
   l.a.g_head = p->heads > 1 ? grad_head_stride : 0;
+  l.a.v = p->v;
+  l.a.v_row = p->kv_rows > 1 ? p->v_row_stride : 0;
+  l.a.v_head = p->kv_heads > 1 ? p->v_head_stride : 0;
   l.a.bstats = reinterpret_cast<float4*>(ws);
+  l.a.norms = reinterpret_cast<float2*>(ws + w.norms);
+  l.a.norm_parts = attn_delta_grid(l);
   l.a.dq = dq;
   l.a.dk = dk;
   l.a.dv = dv;

@@ -41,10 +41,53 @@ enum : int { KERNEL_DQ = 5, KERNEL_DKV = 6, KERNEL_DBIAS = 7 };
 constexpr int kBwdThreads = 576;
 constexpr int kTmaWarp = 16, kMmaWarp = 17, kElemWarps = 16;
 
+// fp16 has 11 bits from 2^-14 to 65504 and loses them below. dS is about |g| / keys, and the weights
+// of many keys are as small, so in fp16 both are formed times a power of two that the stores take
+// out again; it enters exponents and constants that are there anyway. Weights are at most 1 (1.02
+// where a bias puts the scores far from 0): P^T of dkv times 2^14. |dp - d| <= |g| (|v| + |o|), and o
+// is a mean of rows of V: times 2^lift(|g|, largest |v|), |.| the norm of a row, dS stays below
+// 2^15.1. dq takes each row's own |g|; dkv, whose sums run over queries, the largest. 4096 keys, dim
+// 64, gradients of 1e-3: dq was off by 8 times the rounding of the result, now 1.4. bf16 has the
+// exponents of fp32 and needs none of this. It costs fp16 3 to 4 % of a step (ragged batch of 8192
+// rows, 12 heads on 6 of 64: 289 -> 300 us; one sequence of 8192, 16 on 4 of 128: 1550 -> 1586).
+constexpr int kLiftP = 14;
+template <typename T>
+constexpr bool kLift = !IsBf16<T>::v;
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ int lift(float g, float v) {
+  const float x = g * v;      // 2^k <= x < 2^(k + 1), so 2.02 x < 2^(k + 2.1)
+  const int k = (__float_as_int(x) >> 23) - 127;
+  return x > 0.f && x < 1e38f ? min(13 - k, 60) : 0;      // (rows that are not finite: nothing to keep)
+}
+// the largest row norms of g and v, from the delta kernel's parts; all threads of the block, red: two
+// words of shared memory that are 0
+__device__ __forceinline__ float2 largest_norms(const AttnArgs& a, int* red) {
+  float g = 0.f, v = 0.f;
+  for (int i = threadIdx.x; i < a.norm_parts; i += blockDim.x) {
+    g = fmaxf(g, a.norms[i].x);
+    v = fmaxf(v, a.norms[i].y);
+  }
+  const uint32_t wg = __reduce_max_sync(0xffffffffu, __float_as_uint(g));   // not negative: ordered like
+  const uint32_t wv = __reduce_max_sync(0xffffffffu, __float_as_uint(v));   // their bits
+  if ((threadIdx.x & 31) == 0) {
+    atomicMax(red, static_cast<int>(wg));
+    atomicMax(red + 1, static_cast<int>(wv));
+  }
+  __syncthreads();
+  return make_float2(__int_as_float(red[0]), __int_as_float(red[1]));
+}
+
+// first and behind-last row that belong to a sequence
+__device__ __forceinline__ void rows_inside(const AttnArgs& a, const int* cu, int rows, int& lo, int& hi) {
+  lo = cu ? min(max(cu[0], 0), rows) : 0;
+  hi = cu ? min(max(cu[a.seqs], lo), rows) : rows;
+}
+
 // bstats[head][row], so that a tile's are read in whole lines: without a bias
 // x = m c + log2(l) with c = scale log2(e), so that p = 2^(c s - x); with one x = m, y = log2(l), p = 2^((t - x) log2(e) - y), which stays
 // exact for scores near the type's lowest value. z = rowsum(g * o). A row without keys has
-// log2(l) = inf, hence p = 0.
+// log2(l) = inf, hence p = 0. In fp16 w = |g| of the row, and the block's largest norms of g and v
+// go to `norms`; masked keys and rows of no sequence, which may hold anything, do not count.
 template <typename T>
 __global__ void __launch_bounds__(256)
 attn_delta_kernel(const __grid_constant__ AttnArgs a, int lanes, int bias) {
@@ -52,10 +95,13 @@ attn_delta_kernel(const __grid_constant__ AttnArgs a, int lanes, int bias) {
   const long long n = static_cast<long long>(a.q_rows) * a.heads;
   const int per = blockDim.x / lanes, l = threadIdx.x % lanes;
   const float c = log2_scale(a.scale);
+  float top_g = 0.f, top_v = 0.f;
+  int lo = 0, hi = 0;
+  if (kLift<T>) rows_inside(a, a.cu_q, a.q_rows, lo, hi);
   // the bound is the same for all threads of a warp: the sums below exchange lanes
   for (long long i0 = static_cast<long long>(blockIdx.x) * per; i0 < n; i0 += static_cast<long long>(gridDim.x) * per) {
     const long long i = i0 + threadIdx.x / lanes;
-    float s = 0.f;
+    float s = 0.f, gg = 0.f;
     if (i < n && l * 8 < a.dim) {
       const long long row = i / a.heads;
       const int head = static_cast<int>(i - row * a.heads);
@@ -67,12 +113,48 @@ attn_delta_kernel(const __grid_constant__ AttnArgs a, int lanes, int bias) {
               IsBf16<T>::v, y);
 #pragma unroll
       for (int k = 0; k < 8; ++k) s = fmaf(x[k] + z[k], y[k], s);
+      if (kLift<T>)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) gg = fmaf(y[k], y[k], gg);
     }
-    for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    for (int o = lanes / 2; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (kLift<T>) gg += __shfl_xor_sync(0xffffffffu, gg, o);
+    }
     if (i < n && l == 0) {
       const float2 st = a.stats[i];
-      a.bstats[static_cast<size_t>(i % a.heads) * a.q_rows + i / a.heads] = bias ? make_float4(st.x, st.y, s, 0.f) : make_float4(fmaf(st.x, c, st.y), 0.f, s, 0.f);
+      const float w = kLift<T> ? sqrtf(gg) : 0.f;
+      if (kLift<T> && w < 1e38f && i / a.heads >= lo && i / a.heads < hi) top_g = fmaxf(top_g, w);
+      a.bstats[static_cast<size_t>(i % a.heads) * a.q_rows + i / a.heads] = bias ? make_float4(st.x, st.y, s, w) : make_float4(fmaf(st.x, c, st.y), 0.f, s, w);
     }
+  }
+  if (kLift<T>) {
+    const long long nv = static_cast<long long>(a.kv_rows) * a.kv_heads;
+    rows_inside(a, a.cu_k, a.kv_rows, lo, hi);
+    for (long long i0 = static_cast<long long>(blockIdx.x) * per; i0 < nv; i0 += static_cast<long long>(gridDim.x) * per) {
+      const long long i = i0 + threadIdx.x / lanes, row = i / a.kv_heads;
+      float vv = 0.f;
+      if (i < nv && l * 8 < a.dim && row >= lo && row < hi && !(a.key_mask && a.key_mask[row] == 0)) {
+        float y[8];
+        unpack8(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + row * a.v_row + (i - row * a.kv_heads) * a.v_head + l * 8),
+                IsBf16<T>::v, y);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) vv = fmaf(y[k], y[k], vv);
+      }
+      for (int o = lanes / 2; o > 0; o >>= 1) vv += __shfl_xor_sync(0xffffffffu, vv, o);
+      if (vv < 1e38f) top_v = fmaxf(top_v, sqrtf(vv));
+    }
+    __shared__ int red[2];
+    if (threadIdx.x < 2) red[threadIdx.x] = 0;
+    __syncthreads();
+    const uint32_t wg = __reduce_max_sync(0xffffffffu, __float_as_uint(top_g));
+    const uint32_t wv = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
+    if ((threadIdx.x & 31) == 0) {
+      atomicMax(red, static_cast<int>(wg));
+      atomicMax(red + 1, static_cast<int>(wv));
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) a.norms[blockIdx.x] = make_float2(__int_as_float(red[0]), __int_as_float(red[1]));
   }
   grid_dep_release();
 }
@@ -198,11 +280,13 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
   uint64_t* acc_full = q_full + 18;
   uint64_t* drain = q_full + 19;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 20);
+  int* red = reinterpret_cast<int*>(tmem_slot + 1);   // 2
 
   const int warp = uniform<E>(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 20; ++i) mbar_init(q_full + i, i == 13 || i == 17 ? kElemWarps : 1);
     fence_mbar_init();
+    red[0] = red[1] = 0;
   }
   if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
@@ -211,6 +295,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
   const uint32_t tmem = uniform<E>(*tmem_slot);
   grid_dep_wait();
   grid_dep_release();
+  const float top_v = kLift<T> ? largest_norms(a, red).y : 0.f;
   // columns: S of even tiles 0, dP 128, dQ 256, S of odd tiles 384
   int n = blockIdx.x;
   Item it;
@@ -354,7 +439,8 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       const int seen = a.causal ? min(it.klen, it.pos0 + tok + it.off + 1) : it.klen;
       const float4 st = live ? a.bstats[static_cast<size_t>(it.head * a.group + gi) * a.q_rows + it.q0 + tok]
                              : make_float4(0.f, INFINITY, 0.f, 0.f);
-      const float ref = BIAS || live ? st.x : INFINITY;
+      const int up = kLift<T> ? lift(st.w, top_v) : 0;
+      const float ref = BIAS ? st.x : live ? st.x - up : INFINITY, ylift = st.y - up;
       for (int kt = it.kt0; kt < it.kt1; ++kt, ++kn) {
         const int b = kn & 1;
         const uint32_t on = (a.key_mask ? key_word(a, it, kt, part, lane) : 0xffffffffu) &
@@ -375,7 +461,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const float x = __uint_as_float(r[e]);
-          r[e] = __float_as_uint(ex2(BIAS ? fmaf(x - ref, kLog2e, -st.y) : fmaf(x, c, -ref)));
+          r[e] = __float_as_uint(ex2(BIAS ? fmaf(x - ref, kLog2e, -ylift) : fmaf(x, c, -ref)));
         }
         if (cut) {
 #pragma unroll
@@ -408,7 +494,13 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
           // transposed in shared memory, so that a warp writes neighbours of one row at a time
           uint32_t* tile = reinterpret_cast<uint32_t*>(smem + C::kOffT) + warp * 32 * 17;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) tile[lane * 17 + e] = pk[e];
+          for (int e = 0; e < 16; ++e) {
+            if (kLift<T>) {   // exact, or a subnormal
+              const float2 f = unpack2<T>(pk[e]);
+              pk[e] = pack16<T>(f.x * pow2(-up), f.y * pow2(-up));
+            }
+            tile[lane * 17 + e] = pk[e];
+          }
           __syncwarp();
           const int col = kt * kTileRows + part * 32 + lane, row0 = it.pos0 + quad * 32;
           if (col < a.k_len) {
@@ -430,7 +522,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
         ++qn;
         tc_fence_after();
       }
-      store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, a.scale, live && ok, any, dq + orow * a.dim);
+      store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, a.scale * pow2(-up), live && ok, any, dq + orow * a.dim);
       tc_fence_before();
     }
   }
@@ -486,12 +578,14 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   uint64_t* acc_full = kv_full + 20;
   uint64_t* drain = kv_full + 21;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_full + 22);
+  int* red = reinterpret_cast<int*>(tmem_slot + 1);   // 2
 
   const int warp = uniform<E>(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 22; ++i)
       mbar_init(kv_full + i, i == 11 || i == 14 || i == 15 || i == 17 || i == 19 ? kElemWarps : 1);
     fence_mbar_init();
+    red[0] = red[1] = 0;
   }
   // rows of a query tile that no load writes (128 is no multiple of the group): zero once
   {
@@ -509,6 +603,12 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
   const uint32_t tmem = uniform<E>(*tmem_slot);
   grid_dep_wait();
   grid_dep_release();
+  int up = 0;      // of dS^T; P^T, which it is formed of, has 2^kLiftP in it
+  if (kLift<T>) {
+    const float2 top = largest_norms(a, red);
+    up = lift(top.x, top.y);
+  }
+  const float rest = kLift<T> ? pow2(up - kLiftP) : 1.f;
   // columns: S^T / P^T 0, dP^T / dS^T 128, dV 256, dK 384
   int n = blockIdx.x;
   Item it;
@@ -567,6 +667,10 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           const bool live = col_tok[w] < left;
           const size_t at = live ? static_cast<size_t>(it.head) * a.group * a.q_rows + it.q0 + t * a.tq + col_off[w] : 0;
           st[w] = a.bstats[at];
+          if (kLift<T>) {
+            (BIAS ? st[w].y : st[w].x) -= kLiftP;
+            st[w].z *= rest;
+          }
           if (!live) st[w] = make_float4(BIAS ? 0.f : INFINITY, INFINITY, 0.f, 0.f);   // p = 0
         }
         const int cn = qn - 1, cb = cn % C::kCols;
@@ -760,7 +864,8 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           float x[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            x[k] = __uint_as_float(r[e + k]) * (__uint_as_float(d[e + k]) - zs[k]);
+            const float y = kLift<T> ? fmaf(__uint_as_float(d[e + k]), rest, -zs[k]) : __uint_as_float(d[e + k]) - zs[k];
+            x[k] = __uint_as_float(r[e + k]) * y;
             if (cut) x[k] = r[e + k] ? x[k] : 0.f;
           }
           pk[e / 2] = pack16<T>(x[0], x[1]);
@@ -783,14 +888,15 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         ++in;
         tc_fence_after();
       }
+      const float fk = a.scale * pow2(-up), fv = kLift<T> ? pow2(-kLiftP) : 1.f;
       if (a.kv_splits > 1) {
         const size_t all = static_cast<size_t>(a.kv_rows) * a.kv_heads * a.dim;
         float* to = a.dkv_part + 2 * it.slot * all + orow * a.dim;
-        store_part<DP / 4>(lanes + 384, part * (DP / 4), a.dim, a.scale, live && ok, any, to);
-        store_part<DP / 4>(lanes + 256, part * (DP / 4), a.dim, 1.f, live && ok, any, to + all);
+        store_part<DP / 4>(lanes + 384, part * (DP / 4), a.dim, fk, live && ok, any, to);
+        store_part<DP / 4>(lanes + 256, part * (DP / 4), a.dim, fv, live && ok, any, to + all);
       } else {
-        store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, 1.f, live && ok, any, dv + orow * a.dim);
-        store_acc<DP / 4>(lanes + 384, part * (DP / 4), a.dim, a.scale, live && ok, any, dk + orow * a.dim);
+        store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, fv, live && ok, any, dv + orow * a.dim);
+        store_acc<DP / 4>(lanes + 384, part * (DP / 4), a.dim, fk, live && ok, any, dk + orow * a.dim);
       }
       tc_fence_before();
     }
@@ -1065,11 +1171,17 @@ cudaError_t go(Kern kern, const AttnLaunch& l, int grid, int smem) {
 
 }  // namespace
 
+// Threads that share a row of the delta kernel, and its blocks: 8 per SM at most.
+static int delta_lanes(const AttnLaunch& l) { return l.a.dim <= 32 ? 4 : l.a.dim <= 64 ? 8 : 16; }
+int attn_delta_grid(const AttnLaunch& l) {
+  const long long per = 256 / delta_lanes(l), n = static_cast<long long>(l.a.q_rows) * l.a.heads;
+  const long long need = (n + per - 1) / per, cap = static_cast<long long>(l.sms) * kDeltaBlocks;
+  return static_cast<int>(need < cap ? need : cap);
+}
+
 cudaError_t launch_attn_delta(const AttnLaunch& l) {
-  const int lanes = l.a.dim <= 32 ? 4 : l.a.dim <= 64 ? 8 : 16;
-  const long long per = 256 / lanes, n = static_cast<long long>(l.a.q_rows) * l.a.heads;
-  const long long need = (n + per - 1) / per, cap = static_cast<long long>(l.sms) * 8;
-  const dim3 grid(static_cast<unsigned>(need < cap ? need : cap));
+  const int lanes = delta_lanes(l);
+  const dim3 grid(attn_delta_grid(l));
   if (l.bf16) return launch_pdl(attn_delta_kernel<__nv_bfloat16>, grid, dim3(256), 0, l.stream, nullptr, 0, l.a, lanes, l.bias);
   return launch_pdl(attn_delta_kernel<__half>, grid, dim3(256), 0, l.stream, nullptr, 0, l.a, lanes, l.bias);
 }

@@ -49,3 +49,115 @@ def test_keys_times_the_heads_of_a_group_pass_32_bits():
     for name, a, want, off in zip(("o", "dq", "dk", "dv"), got, (w.o, w.dq, w.dk, w.dv),
                                   (w.eo, w.edq, w.edk, w.edv)):
         ref.close(a, want, off, name)
+
+
+# ------------------------------------------------------------------- gradients of any size in fp16
+def exact(q, k, v, g, bias=None, keep=None, scale=None):
+    """dq, dk, dv (and dbias) in 64 bits; q, k, v, g (..., length, dim), grouped heads repeated."""
+    x = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    b = None if bias is None else bias.detach().double().requires_grad_()
+    s = x[0] @ x[1].transpose(-1, -2) * (q.shape[-1] ** -0.5 if scale is None else scale)
+    if b is not None:
+        s = s + b
+    if keep is not None:
+        s = s.masked_fill(~keep, -torch.inf)
+    return torch.autograd.grad(s.softmax(-1) @ x[2], x if b is None else [*x, b], g.double())
+
+
+def roundings(got, want):
+    """The error's norm over that of the result's own rounding (subnormal steps included)."""
+    assert not got.isnan().any() and not got.isinf().any()
+    return ((got.double() - want).norm() / (want.to(got.dtype).double() - want).norm()).item()
+
+
+# dS, or the weights, and the result are each rounded once, independently and by the same relative
+# size: sqrt(2) = 1.41 times the result's rounding alone, and nearer to 1 where the result itself is
+# subnormal. 1.5 leaves 6 % for the spread over the elements.
+MOST = 1.5
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-4, 1e3])
+@pytest.mark.parametrize("d", [64, 128])
+def test_fp16_gradients_of_any_size(size, d):
+    from fast_trimul_b200.functional import packed_attention
+    nq, nk, h = 256, 4096, 2
+    r = gen(2)
+    q, k, v, g = r(nq, h, d).to(HF), r(nk, h, d).to(HF), r(nk, h, d).to(HF), (size * r(nq, h, d)).to(HF)
+    got = train(packed_attention, (q, k, v), g, ends([nq]), ends([nk]), causal=False)
+    want = exact(*(t.transpose(0, 1) for t in (q, k, v, g)))
+    for name, a, b in zip(("dq", "dk", "dv"), got[1:], want):
+        assert roundings(a, b.transpose(0, 1)) <= MOST, name
+
+
+def test_fp16_weights_of_many_keys():
+    """Weights below fp16's normal numbers: 2^-15 on average."""
+    from fast_trimul_b200.functional import packed_attention
+    nq, nk, h, d = 128, 32768, 1, 64
+    r = gen(3)
+    q, k, v, g = r(nq, h, d).to(HF), r(nk, h, d).to(HF), r(nk, h, d).to(HF), r(nq, h, d).to(HF)
+    got = train(packed_attention, (q, k, v), g, ends([nq]), ends([nk]), causal=False)
+    want = exact(*(t.transpose(0, 1) for t in (q, k, v, g)))
+    for name, a, b in zip(("dq", "dk", "dv"), got[1:], want):
+        assert roundings(a, b.transpose(0, 1)) <= MOST, name
+
+
+def test_fp16_gradients_of_a_scaled_loss_do_not_overflow():
+    """dS far above 65504 between operands and results that fp16 holds."""
+    from fast_trimul_b200.functional import packed_attention
+    nq, nk, h, d = 64, 4, 2, 64
+    r = gen(4)
+    q, k = (0.01 * r(nq, h, d)).to(HF), (0.01 * r(nk, h, d)).to(HF)
+    v, g = (10 * r(nk, h, d)).to(HF), (4000 * r(nq, h, d)).to(HF)
+    got = train(packed_attention, (q, k, v), g, ends([nq]), ends([nk]), causal=False)
+    want = exact(*(t.transpose(0, 1) for t in (q, k, v, g)))
+    for name, a, b in zip(("dq", "dk", "dv"), got[1:], want):
+        assert roundings(a, b.transpose(0, 1)) <= MOST, name
+
+
+def test_fp16_sequences_whose_gradients_differ_in_size():
+    from fast_trimul_b200.functional import packed_attention
+    n, h, d = 1024, 2, 64
+    r = gen(5)
+    q, k, v, g = (r(2 * n, h, d).to(HF) for _ in range(4))
+    g[n:] *= 1e-3
+    got = train(packed_attention, (q, k, v), g, ends([n, n]))
+    keep = torch.ones(n, n, dtype=torch.bool, device="cuda").tril()
+    for at in (slice(0, n), slice(n, 2 * n)):
+        want = exact(*(t[at].transpose(0, 1) for t in (q, k, v, g)), keep=keep)
+        for name, a, b in zip(("dq", "dk", "dv"), got[1:], want):
+            assert roundings(a[at], b.transpose(0, 1)) <= MOST, (name, at)
+
+
+@pytest.mark.parametrize("r, n, d", [(1, 500, 24), (6, 300, 32), (1, 300, 96), (5, 200, 128)])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 300.0])
+def test_fp16_gradients_of_any_size_with_a_bias(r, n, d, size):
+    # the bias' gradient is rounded once more at most (one row alone: dS and its step down)
+    from fast_trimul_b200.functional import pair_attention
+    x = gen(6)
+    q, k, v = x(1, r, n, 3, 2, d).to(HF).unbind(3)
+    bias, g = x(1, 2, n, n).to(HF), (size * x(1, r, n, 2, d)).to(HF)
+    got = train(pair_attention, (q, k, v, bias), g)
+    want = exact(*(t.transpose(2, 3) for t in (q, k, v, g)), bias=bias.unsqueeze(1))
+    for name, a, b in zip(("dq", "dk", "dv"), got[1:], want):
+        assert roundings(a, b.transpose(2, 3)) <= MOST, name
+    assert roundings(got[4], want[3].squeeze(1)) <= MOST, "dbias"
+
+
+def test_fp16_rows_that_do_not_count_change_nothing():
+    """Masked keys, and rows of no sequence, may hold anything: the same bits."""
+    from fast_trimul_b200.functional import packed_attention
+    lens, h, d = [200, 131], 2, 64
+    n = sum(lens)
+    r = gen(7)
+    q, k, v, g = (r(n + 20, h, d).to(HF) for _ in range(4))
+    g *= 1e-3
+    mask = torch.rand(n + 20, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) > 0.3
+    cu = ends(lens, 10)
+    want = train(packed_attention, (q, k, v), g, cu, key_mask=mask)
+    for bad in (float("nan"), float("inf"), 65504.0):
+        k2, v2, q2, g2 = k.clone(), v.clone(), q.clone(), g.clone()
+        for t in (k2, v2, q2, g2):
+            t[:10], t[n + 10:] = bad, bad
+        k2[~mask], v2[~mask] = bad, bad
+        got = train(packed_attention, (q2, k2, v2), g2, cu, key_mask=mask)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
