@@ -91,6 +91,15 @@ variable_list once(variable_list grads, const variable_list& from) {
   return out;
 }
 
+// Forward-mode derivatives are not formed. Below autograd a dual tensor's tangent would be lost, and
+// a result without one is read as a derivative of zero.
+void no_tangent(std::initializer_list<const Tensor*> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(),
+                "layer norm and attention of fast_trimul_b200 have no forward-mode derivatives on a GPU");
+}
+
 bool capturing() { return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; }
 
 // A leaf whose gradients an eager graph that still lives collects on the default stream. A
@@ -157,6 +166,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     not_held(ctx->saved_data["held"].toBool());
+    no_tangent({&grads[0]});
     variable_list res = gradients(ctx, grads);
     if (!at::GradMode::is_enabled()) return res;
     const auto saved = ctx->get_saved_variables();
@@ -202,6 +212,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 py::object layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
   int64_t rows, stride;
+  if (x.is_cuda()) no_tangent({&x, given(w), given(b)});
   if (!x.is_cuda() || x.dim() < 1 || x.numel() == 0 || dtype_of(x) < 0 || !(eps >= 0) || !rows_of(x, rows, stride) ||
       x.size(-1) > INT_MAX)
     return py::none();
@@ -326,6 +337,7 @@ struct Attention : torch::autograd::Function<Attention> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     not_held(ctx->saved_data["held"].toBool());
+    no_tangent({&grads[0]});
     variable_list res = gradients(ctx, grads);
     if (!at::GradMode::is_enabled()) return res;
     const auto saved = ctx->get_saved_variables();
@@ -415,6 +427,7 @@ bool mask_ok(const OptTensor& m, const Tensor& q, at::IntArrayRef shape) {
 
 py::object packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k,
                   bool causal, std::optional<double> scale, const OptTensor& mask) {
+  no_tangent({&q, &k, &v});
   if (q.dim() != 3 || k.dim() != 3 || v.dim() != 3 || q.size(2) != k.size(2)) return py::none();
   const double s = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2)));
   if (k.size(1) < 1 || !plain(q, k, v, s, q.size(1), k.size(1), q.size(2)) || !index_ok(cu_q, q) ||
@@ -433,6 +446,7 @@ py::object packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
 
 py::object cached(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths,
                   std::optional<double> scale) {
+  no_tangent({&q, &k, &v});
   if (q.dim() != 3 || k.dim() != 4 || v.dim() != 4 || q.size(0) != k.size(0) || q.size(2) != k.size(3))
     return py::none();
   const double s = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2)));
@@ -451,6 +465,7 @@ py::object cached(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
 
 py::object pair(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias, const OptTensor& mask,
                 std::optional<double> scale) {
+  no_tangent({&q, &k, &v, given(bias)});
   if (q.dim() != 5 || k.sizes() != q.sizes() || v.sizes() != q.sizes()) return py::none();
   const int64_t B = q.size(0), R = q.size(1), N = q.size(2), H = q.size(3), D = q.size(4);
   const double s = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(D));

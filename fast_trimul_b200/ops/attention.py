@@ -13,7 +13,8 @@ of a pair representation with a shared bias.
 On CUDA tensors the kernels take fp16 and bf16 with a head dimension that is a multiple of 8
 up to 128, and raise `NativeDeclined` for anything else; sums, softmax statistics and
 gradients' accumulators are fp32. Elsewhere the formula runs in torch, in fp32. A query that
-sees no key gives zeros, and masked keys count as absent whatever K and V hold there.
+sees no key gives zeros, and masked keys count as absent whatever K and V hold there. The kernels
+have first derivatives in reverse mode only; second ones and tangents (forward mode) are refused.
 """
 
 import ctypes

@@ -44,9 +44,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(variance + eps) * weight + bias over x's last dimension.
 
     x: (..., width) fp32, fp16 or bf16; weight, bias: (width,) of any of these types, or
-    None. Returns x's shape and type. Differentiable once in x, weight and bias; the
-    gradients have their inputs' types and are the same bits on every call. Rows may be
-    strided (a slice of a wider tensor is read in place); other layouts are copied first."""
+    None. Returns x's shape and type. Differentiable once in x, weight and bias (tangents,
+    of forward mode, are refused on a GPU); the gradients have their inputs' types and are
+    the same bits on every call. Rows may be strided (a slice of a wider tensor is read in
+    place); other layouts are copied first."""
     if x.is_cuda:
         try:
             out = _lib.torch_ext().layer_norm(x, weight, bias, eps)

@@ -161,3 +161,52 @@ def test_fp16_rows_that_do_not_count_change_nothing():
         k2[~mask], v2[~mask] = bad, bad
         got = train(packed_attention, (q2, k2, v2), g2, cu, key_mask=mask)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# -------------------------------------------------------------------- derivatives that are not formed
+def operators():
+    """Each operator with inputs, for the calls below: name, call, tensors."""
+    from fast_trimul_b200.functional import cached_attention, layer_norm, packed_attention, pair_attention
+    r = gen(8)
+    t = lambda *s: r(*s).to(BF)   # noqa: E731
+    lens = torch.tensor([5, 3], dtype=torch.int32, device="cuda")
+    return [("layer_norm", layer_norm, [t(5, 64), r(64), r(64)]),
+            ("layer_norm, copied", lambda x, w, b: layer_norm(x.transpose(0, 1), w, b), [t(64, 5), r(64), r(64)]),
+            ("packed", lambda *x: packed_attention(*x, ends([40])), [t(40, 2, 32) for _ in range(3)]),
+            ("pair", pair_attention, [t(1, 2, 24, 2, 32) for _ in range(3)] + [t(1, 2, 24, 24)]),
+            ("cached", lambda *x: cached_attention(*x, lens), [t(2, 4, 32), t(2, 9, 2, 32), t(2, 9, 2, 32)])]
+
+
+@pytest.mark.parametrize("op", range(5))
+def test_forward_mode_derivatives_are_refused(op):
+    # a result without a tangent would be read as a derivative of zero
+    import torch.autograd.forward_ad as fwd
+    name, f, inputs = operators()[op]
+    for i in range(len(inputs)):
+        with fwd.dual_level():
+            x = list(inputs)
+            x[i] = fwd.make_dual(x[i], torch.ones_like(x[i]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f(*x)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                f(*x)
+            if name != "cached":
+                y = [t.detach().clone().requires_grad_() for t in inputs]
+                y[i] = fwd.make_dual(y[i], torch.ones_like(y[i]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f(*y)
+        f(*inputs)                   # and without the tangent it runs
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(f, tuple(inputs), tuple(torch.ones_like(t) for t in inputs))
+
+
+@pytest.mark.parametrize("op", range(4))
+def test_a_gradient_with_a_tangent_is_refused(op):
+    import torch.autograd.forward_ad as fwd
+    _, f, inputs = operators()[op]
+    leaves = [t.detach().clone().requires_grad_() for t in inputs]
+    with fwd.dual_level():
+        out = f(*leaves)
+        g = fwd.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, leaves, g)
