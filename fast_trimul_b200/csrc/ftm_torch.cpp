@@ -91,6 +91,15 @@ variable_list once(variable_list grads, const variable_list& from) {
   return out;
 }
 
+// A tensor without elements at `t`'s place in the graph: what a backward keeps of an input whose
+// values it does not need, so that `once` can name it.
+Tensor place_of(const OptTensor& t) {
+  if (!t.has_value() || !t->defined() || !t->requires_grad()) return Tensor();
+  Tensor place = at::empty({0}, t->options());
+  torch::autograd::impl::set_gradient_edge(place, torch::autograd::impl::gradient_edge(*t));
+  return place;
+}
+
 // Forward-mode derivatives are not formed. Below autograd a dual tensor's tangent would be lost, and
 // a result without one is read as a derivative of zero.
 void no_tangent(std::initializer_list<const Tensor*> inputs) {
@@ -327,7 +336,8 @@ struct Attention : torch::autograd::Function<Attention> {
                         const Call& c) {
     Kept t;
     Tensor out = attend(c, q, k, v, c.ready_bias, &t);
-    ctx->save_for_backward({q, k, v, c.ready_bias, out, t.stats, t.lists, c.cu_q, c.cu_k, c.mask, t.low});
+    ctx->save_for_backward({q, k, v, c.ready_bias, out, t.stats, t.lists, c.cu_q, c.cu_k, c.mask, t.low,
+                            place_of(bias)});
     ctx->saved_data["n"] = std::vector<int64_t>{c.seqs, c.q_len, c.kv_len, c.bias_seqs, c.causal};
     ctx->saved_data["scale"] = c.scale;
     ctx->saved_data["held"] = c.held;
@@ -341,7 +351,9 @@ struct Attention : torch::autograd::Function<Attention> {
     variable_list res = gradients(ctx, grads);
     if (!at::GradMode::is_enabled()) return res;
     const auto saved = ctx->get_saved_variables();
-    return once(std::move(res), {grads[0], saved[0], saved[1], saved[2]});
+    variable_list from{grads[0], saved[0], saved[1], saved[2]};
+    if (saved[11].defined()) from.push_back(saved[11]);
+    return once(std::move(res), from);
   }
 
   static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {

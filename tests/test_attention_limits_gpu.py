@@ -210,3 +210,16 @@ def test_a_gradient_with_a_tangent_is_refused(op):
         g = fwd.make_dual(torch.ones_like(out), torch.ones_like(out))
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(out, leaves, g)
+
+
+@pytest.mark.parametrize("n", [24, 25])          # read in place, and padded
+@pytest.mark.parametrize("leaf", [True, False])
+def test_a_second_derivative_in_the_bias_is_refused(n, leaf):
+    from fast_trimul_b200.functional import pair_attention
+    r = gen(9)
+    q, k, v = (r(1, 2, n, 2, 32).to(BF).requires_grad_() for _ in range(3))
+    w = r(1, 2, n, n).to(BF).requires_grad_()
+    bias = w if leaf else w * 2
+    (dq,) = torch.autograd.grad(pair_attention(q, k, v, bias), q, torch.ones_like(q), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(dq.float().sum(), w, allow_unused=True)
