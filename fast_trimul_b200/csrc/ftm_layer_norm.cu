@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kLnThreads = 256;    // block of the warp-row kernels
 constexpr int kLnMaxReg = 8192;    // widest row held in registers
+constexpr int kLnMaxWidth = (1 << 30) - 1024;   // columns of dw and db together are counted in 32 bits
 
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
@@ -497,7 +498,7 @@ using namespace ftm;
 extern "C" {
 
 size_t ftm_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t width) {
-  if (rows < 1 || width < 1) return 0;
+  if (rows < 1 || width < 1 || width > kLnMaxWidth) return 0;
   // at most 1024 / 128 blocks per SM, and never more than rows
   const long long cap = static_cast<long long>(ln_sms()) * 8;
   return static_cast<size_t>(rows < cap ? rows : cap) * 2 * width * sizeof(float);
@@ -507,7 +508,7 @@ int ftm_layer_norm_fwd(const void* x, int32_t dtype, int64_t x_row_stride, const
                        int32_t weight_dtype, const void* bias, int32_t bias_dtype, float eps, void* y,
                        float* stats, int64_t rows, int32_t width, ftm_stream_t stream) {
   if (!x || !y || !(eps >= 0.f)) return FTM_BAD_ARGUMENT;
-  if (rows < 1 || width < 1 || x_row_stride < 0) return FTM_BAD_SHAPE;
+  if (rows < 1 || width < 1 || width > kLnMaxWidth || x_row_stride < 0) return FTM_BAD_SHAPE;
   if (!dt_ok(dtype) || (weight && !dt_ok(weight_dtype)) || (bias && !dt_ok(bias_dtype)))
     return FTM_BAD_DTYPE;
   if (!elem_aligned(x, dtype) || !elem_aligned(y, dtype) || (stats && (reinterpret_cast<uintptr_t>(stats) & 7)))
@@ -529,7 +530,7 @@ int ftm_layer_norm_bwd(const void* x, int32_t dtype, int64_t x_row_stride, const
                        void* workspace, size_t workspace_bytes, int64_t rows, int32_t width,
                        ftm_stream_t stream) {
   if (!x || !grad || !stats || (!dx && !dweight && !dbias)) return FTM_BAD_ARGUMENT;
-  if (rows < 1 || width < 1 || x_row_stride < 0 || grad_row_stride < 0) return FTM_BAD_SHAPE;
+  if (rows < 1 || width < 1 || width > kLnMaxWidth || x_row_stride < 0 || grad_row_stride < 0) return FTM_BAD_SHAPE;
   if (!dt_ok(dtype) || ((weight || dweight) && !dt_ok(weight_dtype)) || (dbias && !dt_ok(dbias_dtype)))
     return FTM_BAD_DTYPE;
   if (!elem_aligned(x, dtype) || !elem_aligned(grad, dtype) || (dx && !elem_aligned(dx, dtype)) ||

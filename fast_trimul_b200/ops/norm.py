@@ -43,7 +43,28 @@ def _formula(x, weight, bias, eps):
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(variance + eps) * weight + bias over x's last dimension.
 
-    x: (..., width) fp32, fp16 or bf16; weight, bias: (width,) of any of these types, or
+    x: (..., width) fp32, fp16 or bf16, on a GPU of at most 2^30 - 1024 columns; weight, bias:
+    (width,) of any of these types, or None. Returns x's shape and type. Differentiable once in
+    x, weight and bias (tangents, of forward mode, are refused on a GPU); the gradients have
+    their inputs' types and are the same bits on every call. Rows may be strided (a slice of a
+    wider tensor is read in place); other layouts are copied first."""
+    if x.is_cuda:
+        for name, p in (("x", x), ("weight", weight), ("bias", bias)):
+            if p is not None and p.dtype not in _DT:
+                raise _lib.NativeDeclined(f"layer_norm takes fp32, fp16 and bf16, got {p.dtype} for {name}")
+
+
+def _formula(x, weight, bias, eps):
+    if all(p is None or p.dtype == x.dtype for p in (weight, bias)):
+        return F.layer_norm(x, (x.shape[-1],), weight, bias, eps)
+    f = lambda p: None if p is None else p.float()   # noqa: E731
+    return F.layer_norm(x.float(), (x.shape[-1],), f(weight), f(bias), eps).to(x.dtype)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(variance + eps) * weight + bias over x's last dimension.
+
+    x: (..., width) fp32, fp16 or bf16, on a GPU of at most 2^30 - 1024 columns; weight, bias: (width,) of any of these types, or
     None. Returns x's shape and type. Differentiable once in x, weight and bias (tangents,
     of forward mode, are refused on a GPU); the gradients have their inputs' types and are
     the same bits on every call. Rows may be strided (a slice of a wider tensor is read in

@@ -332,7 +332,7 @@ int* ftm_static_scratch_error_word(void);
 
 /* ---- layer norm of any width ------------------------------------------------
  * No counterpart in the reference (its layer norms are torch's). Rows of `width`
- * elements `x_row_stride` elements apart (the elements of a row are contiguous; a stride
+ * elements (at most 2^30 - 1024) `x_row_stride` elements apart (a row's are contiguous; a stride
  * of 0 repeats one row); x and y have `dtype`, weight and bias (each may be NULL: 1 and
  * 0) types of their own. y is written contiguously. stats (NULL if no backward follows):
  * 2 * rows floats, (mean, 1 / sqrt(variance + eps)) of each row. Sums are fp32. */
