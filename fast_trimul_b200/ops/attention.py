@@ -165,10 +165,12 @@ def _nothing(like, *inputs):
 
 # --------------------------------------------------------------------------- packed
 def _ends(cu, device, name):
-    if cu.dim() != 1 or cu.numel() < 1 or cu.dtype.is_floating_point or cu.dtype == torch.bool:
+    if cu.dim() != 1 or cu.numel() < 1 or cu.dtype.is_floating_point or cu.dtype.is_complex or cu.dtype == torch.bool:
         raise ValueError(f"{name} must be a vector of whole numbers, got {cu.dtype} {tuple(cu.shape)}")
     if cu.device != device:
         raise ValueError(f"{name} is on {cu.device}, q on {device}")
+    if cu.dtype not in (torch.int8, torch.uint8, torch.int16, torch.int32):   # past 32 bits: past any tensor, too
+        cu = cu.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1)
     return cu.to(torch.int32).contiguous()
 
 

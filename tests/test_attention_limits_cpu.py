@@ -52,3 +52,17 @@ def test_columns_in_front_of_the_first_query(host):
 def test_rows_of_a_query_tile(host):
     rows = [(n, 128 // g, g) for n in FAR[1:] for g in (1, 2, 3, 64, 127, 128)]
     assert host("rows_held", rows) == [min(n, tq) * g for n, tq, g in rows]
+
+
+def test_lengths_past_32_bits_are_clamped_not_wrapped():
+    import torch
+    from fast_trimul_b200.functional import cached_attention
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(*s, generator=g) for s in ((5, 4, 8), (5, 9, 2, 8), (5, 9, 2, 8)))
+    got = cached_attention(q, k, v, torch.tensor([2 ** 31, 2 ** 32 + 3, 2 ** 62, -2 ** 32 + 4, 7]))
+    want = cached_attention(q, k, v, torch.tensor([9, 9, 9, 0, 7], dtype=torch.int32))
+    assert torch.equal(got, want)
+    got = cached_attention(q, k, v, torch.tensor([2 ** 31, 9, 9, 0, 7], dtype=torch.uint32))
+    assert torch.equal(got, want)
+    with pytest.raises(ValueError):
+        cached_attention(q, k, v, torch.ones(5, dtype=torch.complex64))

@@ -223,3 +223,14 @@ def test_a_second_derivative_in_the_bias_is_refused(n, leaf):
     (dq,) = torch.autograd.grad(pair_attention(q, k, v, bias), q, torch.ones_like(q), create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(dq.float().sum(), w, allow_unused=True)
+
+
+def test_lengths_and_ends_past_32_bits_are_clamped_not_wrapped():
+    from fast_trimul_b200.functional import cached_attention, packed_attention
+    r = gen(10)
+    q, k, v = r(3, 4, 32).to(BF), r(3, 140, 2, 32).to(BF), r(3, 140, 2, 32).to(BF)
+    got = cached_attention(q, k, v, torch.tensor([2 ** 32 + 3, 2 ** 31, -2 ** 32 + 4], device="cuda"))
+    assert torch.equal(got, cached_attention(q, k, v, torch.tensor([140, 140, 0], device="cuda")))
+    q, k, v = r(50, 4, 32).to(BF), r(50, 2, 32).to(BF), r(50, 2, 32).to(BF)
+    got = packed_attention(q, k, v, torch.tensor([0, 20, 2 ** 32 + 1], device="cuda"))
+    assert torch.equal(got, packed_attention(q, k, v, ends([20, 30])))
