@@ -350,7 +350,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         ++kn;
       }
     }
-    if (!ok) report_failure(a);
+    if (!ok) report_failure(a, KERNEL_ATTN);
     if (lane == 0) {   // copies in flight land before the block may exit
       if (qn) mbar_wait_drain(q_full, (qn - 1) & 1);
       for (int i = kf > NS ? kf - NS : 0; i < kf; ++i) mbar_wait_drain(&k_full[i % NS], (i / NS) & 1);
@@ -444,7 +444,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       kn += n;
       ++qn;
     }
-    if (!ok) report_failure(a);
+    if (!ok) report_failure(a, KERNEL_ATTN);
     if (issuer<E>(lane)) {
       umma_commit(drain);
       mbar_wait_drain(drain, 0);
@@ -600,6 +600,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         a.stats[orow] = l > 0.f || l != l ? make_float2(m, __log2f(l)) : make_float2(0.f, INFINITY);
       tc_fence_before();   // O read before the next item's first P V is released by p_ready
     }
+    if (!ok) report_failure(a, KERNEL_ATTN);
   }
   __syncwarp();      // the lanes of a role that one lane drained
   __syncthreads();

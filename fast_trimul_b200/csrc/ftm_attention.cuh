@@ -64,11 +64,12 @@ struct AttnArgs {
 };
 
 // a role that gave up tells the host: polling a host word in the waits themselves would cross
-// PCIe on every poll (measured: 50x slower kernels), so only this write goes there
-__device__ __forceinline__ void report_failure(const AttnArgs& a) {
+// PCIe on every poll (measured: 50x slower kernels), so only this write goes there. The device word
+// may have been cleared since; that a kernel gave up is told all the same.
+__device__ __forceinline__ void report_failure(const AttnArgs& a, int kernel) {
   if (a.host_err) {
     const int code = *reinterpret_cast<volatile int*>(a.err);
-    if (code) *reinterpret_cast<volatile int*>(a.host_err) = code;
+    *reinterpret_cast<volatile int*>(a.host_err) = code ? code : err_code(kernel, 0, 0);
     __threadfence_system();
   }
 }

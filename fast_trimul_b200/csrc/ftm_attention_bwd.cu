@@ -416,7 +416,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       }
       ++qn;
     }
-    if (!ok) report_failure(a);
+    if (!ok) report_failure(a, KERNEL_DQ);
     if (issuer<E>(lane)) {
       umma_commit(drain);
       mbar_wait_drain(drain, 0);
@@ -525,6 +525,7 @@ attn_dq_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ At
       store_acc<DP / 4>(lanes + 256, part * (DP / 4), a.dim, a.scale * pow2(-up), live && ok, any, dq + orow * a.dim);
       tc_fence_before();
     }
+    if (!ok) report_failure(a, KERNEL_DQ);
   }
   __syncwarp();      // the lanes of a role that one lane drained
   __syncthreads();
@@ -771,7 +772,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       }
       qn += tiles;
     }
-    if (!ok) report_failure(a);
+    if (!ok) report_failure(a, KERNEL_DKV);
     if (issuer<E>(lane)) {
       umma_commit(drain);
       mbar_wait_drain(drain, 0);
@@ -900,6 +901,7 @@ attn_dkv_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
       }
       tc_fence_before();
     }
+    if (!ok) report_failure(a, KERNEL_DKV);
   }
   __syncwarp();      // the lanes of a role that one lane drained
   __syncthreads();
@@ -1018,7 +1020,7 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
         __syncwarp();
       }
     }
-    if (!ok) report_failure(a);
+    if (!ok) report_failure(a, KERNEL_DBIAS);
     if (issuer<E>(lane)) {
       umma_commit(drain);
       mbar_wait_drain(drain, 0);
@@ -1101,6 +1103,7 @@ attn_dbias_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__
         __syncwarp();
       }
     }
+    if (!ok) report_failure(a, KERNEL_DBIAS);
   }
   __syncwarp();      // the lanes of a role that one lane drained
   __syncthreads();

@@ -47,6 +47,17 @@ struct Words {
 };
 std::array<Words, kMaxGpus> words;
 
+// Failures of each GPU that were cleared, and for each thread how many it knows of (plus one; 0: it
+// has made no call yet, and missed none).
+std::array<std::atomic<unsigned>, kMaxGpus> failures{};
+thread_local std::array<unsigned, kMaxGpus> known{};
+
+bool knows_all(int d) {
+  const unsigned now = failures[d].load() + 1;
+  if (!known[d]) known[d] = now;
+  return known[d] == now;
+}
+
 std::atomic<long> n_calls{0}, n_launches{0};
 
 void count(bool call) {
@@ -424,7 +435,7 @@ bool plain(const Tensor& q, const Tensor& k, const Tensor& v, double scale, int6
       k.numel() == 0 || !(scale >= 0) || !std::isfinite(scale))
     return false;
   const int d = q.get_device();
-  if (d >= kMaxGpus || !words[d].dev || *words[d].host) return false;
+  if (d >= kMaxGpus || !words[d].dev || *words[d].host || !knows_all(d)) return false;
   return heads % kv_heads == 0 && heads / kv_heads <= 128 && dim % 8 == 0 && dim <= 128 && ready(q) && ready(k) &&
          ready(v);
 }
@@ -538,8 +549,23 @@ void bind_library(const std::vector<uintptr_t>& f) {
   set(lib.pad_rows);
 }
 
+void known_gpu(int device) { TORCH_CHECK(device >= 0 && device < kMaxGpus, "device ", device); }
+
+void count_failure(int device) {
+  known_gpu(device);
+  ++failures[device];
+}
+
+// whether a failure was cleared since this thread last asked (or called)
+bool missed_failure(int device) {
+  known_gpu(device);
+  const bool missed = !knows_all(device);
+  known[device] = failures[device].load() + 1;
+  return missed;
+}
+
 void set_words(int device, uintptr_t dev, uintptr_t host) {
-  TORCH_CHECK(device >= 0 && device < kMaxGpus, "device ", device);
+  known_gpu(device);
   words[device].dev = reinterpret_cast<int*>(dev);
   words[device].host = reinterpret_cast<volatile int*>(host);
 }
@@ -549,6 +575,8 @@ void set_words(int device, uintptr_t dev, uintptr_t host) {
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind_library", &bind_library);
   m.def("set_words", &set_words);
+  m.def("count_failure", &count_failure);
+  m.def("missed_failure", &missed_failure);
   m.def("layer_norm", &layer_norm);
   m.def("packed", &packed);
   m.def("cached", &cached);

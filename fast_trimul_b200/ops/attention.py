@@ -30,8 +30,13 @@ _TYPES = (torch.float16, torch.bfloat16)
 
 class AttentionErrorWord:
     """The error words of the attention kernels of one GPU: one on the device, which their waits
-    poll, and one in pinned host memory, which a kernel writes only when a wait expired. The
-    next call (or `check`) sees that with a plain read; no call copies or synchronises."""
+    poll, and one in pinned host memory, which a kernel writes only when it gave up on a wait.
+    The next call (or `check`) sees that with a plain read; no call copies or synchronises.
+
+    Kernels of other streams give up with the one whose wait expired. So every thread that has
+    called before raises once, at its next call or `check`, whichever of them clears the words:
+    the GPU's failures are counted, and each thread compares with the count it saw last (in the
+    extension, which looks at each call)."""
 
     def __init__(self, device):
         if torch.cuda.is_current_stream_capturing():
@@ -40,19 +45,33 @@ class AttentionErrorWord:
         self.host = torch.zeros(16, dtype=torch.int32).pin_memory()
         self.ptr, self.host_ptr = self.dev.data_ptr(), self.host.data_ptr()
         self.word = ctypes.c_int32.from_address(self.host_ptr)
+        self.index, self.code, self.lock = self.dev.device.index, 0, threading.Lock()
         torch.cuda.synchronize(device)     # zeroed, whatever stream reads it first
-        _lib.torch_ext().set_words(self.dev.device.index, self.ptr, self.host_ptr)
+        _lib.torch_ext().set_words(self.index, self.ptr, self.host_ptr)
 
     def poll(self):
-        code = self.word.value
-        if code:
-            if not torch.cuda.is_current_stream_capturing():
-                torch.cuda.synchronize(self.dev.device)   # its kernels have drained
-                self.dev.zero_()
-                self.word.value = 0
-            raise _lib.NativeKernelError(
-                f"a bounded device wait expired in a native attention kernel (code 0x{code:x}: kernel "
-                f"{code >> 8}, role {(code >> 4) & 15}, site {code & 15}); its output is invalid")
+        cleared = False
+        if self.word.value:
+            if torch.cuda.is_current_stream_capturing():
+                self._raise(self.word.value)       # (the words stay set: nothing can be cleared here)
+            with self.lock:
+                if self.word.value:
+                    torch.cuda.synchronize(self.dev.device)   # the kernels that met the error have drained
+                    self.code = self.word.value
+                    self.dev.zero_()
+                    # before the host word: while that is set, other threads' calls come here and wait
+                    torch.cuda.synchronize(self.dev.device)
+                    _lib.torch_ext().count_failure(self.index)
+                    self.word.value = 0
+                    cleared = True
+        if _lib.torch_ext().missed_failure(self.index) or cleared:
+            self._raise(self.code)
+
+    def _raise(self, code):
+        raise _lib.NativeKernelError(
+            f"a bounded device wait expired in a native attention kernel (code 0x{code:x}: kernel "
+            f"{code >> 8}, role {(code >> 4) & 15}, site {code & 15}); attention outputs of this GPU, of any "
+            "stream, that were formed since this thread's last call or check are invalid")
 
     def check(self):
         torch.cuda.synchronize(self.dev.device)

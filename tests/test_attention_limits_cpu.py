@@ -66,3 +66,85 @@ def test_lengths_past_32_bits_are_clamped_not_wrapped():
     assert torch.equal(got, want)
     with pytest.raises(ValueError):
         cached_attention(q, k, v, torch.ones(5, dtype=torch.complex64))
+
+
+# ------------------------------------------------------------------- failures and several threads
+class Calls:
+    """Runs calls in a thread of its own, one after the other."""
+
+    def __init__(self):
+        import concurrent.futures
+        self.pool = concurrent.futures.ThreadPoolExecutor(max_workers=1)
+
+    def __call__(self, f):
+        return self.pool.submit(f).result()
+
+
+@pytest.fixture
+def error_word(monkeypatch):
+    """An AttentionErrorWord without a GPU, and what it does: "synchronize", "zero", "clear" and "count"
+    in order."""
+    import torch
+    from fast_trimul_b200.ops.attention import AttentionErrorWord
+    done = []
+
+    class Dev:
+        device = torch.device("cuda", 63)
+
+        def zero_(self):
+            done.append("zero")
+
+    class Word:
+        now = 0
+
+        @property
+        def value(self):
+            return self.now
+
+        @value.setter
+        def value(self, x):
+            if x == 0:
+                done.append("clear")
+            self.now = x
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: done.append("synchronize"))
+    w = AttentionErrorWord.__new__(AttentionErrorWord)
+    import threading
+    w.dev, w.word, w.index, w.code, w.lock = Dev(), Word(), 63, 0, threading.Lock()
+    return w, done
+
+
+def test_every_thread_that_called_learns_of_a_failure_once(error_word):
+    """Kernels of all streams give up together: who polls first must not be the only one to hear of it."""
+    from fast_trimul_b200 import _lib
+    w, _ = error_word
+    a, b, late = Calls(), Calls(), Calls()
+    a(w.poll)                    # each has called before ...
+    b(w.poll)
+    w.word.now = 0x421           # ... a wait expires ...
+    for thread in (a, b):
+        with pytest.raises(_lib.NativeKernelError, match="0x421"):
+            thread(w.poll)
+        thread(w.poll)           # ... and each hears of it once
+    late(w.poll)                 # a thread that had nothing running hears nothing
+    w.word.now = 0x512
+    with pytest.raises(_lib.NativeKernelError, match="0x512"):
+        late(w.poll)
+    for thread in (a, b):
+        with pytest.raises(_lib.NativeKernelError, match="0x512"):
+            thread(w.poll)
+    fresh = Calls()              # one whose first call finds the word set hears of it, too
+    w.word.now = 0x631
+    with pytest.raises(_lib.NativeKernelError, match="0x631"):
+        fresh(w.poll)
+
+
+def test_the_host_word_is_cleared_last(error_word):
+    """While the device word may still be set, launches of other threads have to find the host word set."""
+    from fast_trimul_b200 import _lib
+    w, done = error_word
+    w.word.now = 0x421
+    with pytest.raises(_lib.NativeKernelError):
+        w.poll()
+    assert done == ["synchronize", "zero", "synchronize", "clear"] and w.word.now == 0

@@ -234,3 +234,36 @@ def test_lengths_and_ends_past_32_bits_are_clamped_not_wrapped():
     q, k, v = r(50, 4, 32).to(BF), r(50, 2, 32).to(BF), r(50, 2, 32).to(BF)
     got = packed_attention(q, k, v, torch.tensor([0, 20, 2 ** 32 + 1], device="cuda"))
     assert torch.equal(got, packed_attention(q, k, v, ends([20, 30])))
+
+
+# ------------------------------------------------------------------- failures and several threads
+def test_a_failure_is_reported_to_every_thread_once(monkeypatch):
+    """A withheld tile of one thread's call: its waits expire, kernels of all streams give up, and the
+    other thread hears of it at its next call as well; afterwards both get right results."""
+    import concurrent.futures
+    from fast_trimul_b200 import _lib
+    from fast_trimul_b200.functional import packed_attention
+    r = gen(11)
+    q, k, v = (r(64, 2, 64).to(BF) for _ in range(3))
+    cu, side = ends([64]), torch.cuda.Stream()
+    want = packed_attention(q, k, v, cu)
+    torch.cuda.synchronize()
+
+    def other():
+        with torch.cuda.stream(side):
+            out = packed_attention(q, k, v, cu)
+        side.synchronize()
+        return out
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=1) as pool:
+        assert torch.equal(pool.submit(other).result(), want)
+        monkeypatch.setenv("FTM_TEST_STALL", "attention")
+        packed_attention(q, k, v, cu)
+        monkeypatch.delenv("FTM_TEST_STALL")
+        torch.cuda.synchronize()
+        with pytest.raises(_lib.NativeKernelError):
+            packed_attention(q, k, v, cu)
+        assert torch.equal(packed_attention(q, k, v, cu), want)
+        with pytest.raises(_lib.NativeKernelError):
+            pool.submit(other).result()
+        assert torch.equal(pool.submit(other).result(), want)
