@@ -518,6 +518,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           }
           if (kt > it.kt0) {
             pv_wait();
+            __syncwarp();
 #pragma unroll 1
             for (int q = 0; q * 32 < a.dim; ++q) {
               uint32_t o[32];
@@ -538,6 +539,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(s_empty);
+          __syncwarp();
         };
         if (far) l += row_weights<true, 1, T>(lanes, lanes + C::kColP, c, ref, pv_wait, all_read);
         else l += row_weights<false, C::kUnroll, T>(lanes, lanes + C::kColP, c, ref, pv_wait, all_read);
@@ -562,6 +564,7 @@ attn_fwd_kernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
 #pragma unroll 1
       for (int q = 0; q * 32 < a.dim; ++q) {
         uint32_t o[32];
+        __syncwarp();
         if (any) {
           FTM_TMEM_LD32_NOWAIT(lanes + 128 + q * 32, o);
           tmem_wait_ld();

@@ -190,10 +190,13 @@ __device__ __forceinline__ bool named_barrier_all(int id, int nthreads, bool ok)
       : "=r"(all)
       : "r"(id), "r"(nthreads), "r"(ok ? 1 : 0)
       : "memory");
+  __syncwarp();
   return all != 0;
 }
 
 // ------------------------------------------------------------------- tcgen05 forms
+// TMEM loads, stores and (de)allocations are instructions of a whole warp (.sync.aligned). Behind a
+// branch that some lanes take alone the lanes meet first: by a vote on a wait, else by __syncwarp().
 // D (+)= A[tmem] * B[smem desc]; A: 16-bit pairs, 8 columns per 16-element step
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
                                             uint32_t idesc, uint32_t accumulate) {
@@ -264,9 +267,12 @@ constexpr int kBlk = kTileRows * 128;   // bytes of one 64-element block
 // per issued MMA, 950 for one P V, which bound the whole kernel. The lanes meet first: an
 // election among some of them would pick another lane, whose commits do not cover the MMAs of
 // the first one.
-// E: which of the two. The kernels with a bias at DP = 128 keep lane 0: with the election they
-// ended with an illegal address that neither reading nor checks of every descriptor and TMEM
-// address explained, so they stay in the form that was tested.
+// E: which of the two. The kernels with a bias at DP = 128 keep lane 0: with the election they once
+// ended with an illegal address whose cause is not known. It was none of the addresses: their
+// matrix instructions take the same ones as without a bias at DP = 128, where the elected form
+// runs, and a check of every descriptor and TMEM address found none out of range. Lanes that a
+// branch had parted could then reach TMEM accesses one after the other, which is undefined; that is
+// mended in all kernels. The kernels with a bias stay in the form that was tested.
 template <bool E>
 __device__ __forceinline__ bool issuer(int lane) {
   if (!E) return lane == 0;

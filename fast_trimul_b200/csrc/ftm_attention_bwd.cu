@@ -176,6 +176,7 @@ __device__ __forceinline__ void store_acc(uint32_t taddr, int col0, int dim, flo
 #pragma unroll
   for (int q = 0; q < COLS / 16; ++q) {
     uint32_t o[16];
+    __syncwarp();
     if (any) {
       tmem_ld16_nowait(taddr + col0 + q * 16, o);
       tmem_wait_ld();
@@ -203,6 +204,7 @@ __device__ __forceinline__ void store_part(uint32_t taddr, int col0, int dim, fl
 #pragma unroll
   for (int q = 0; q < COLS / 16; ++q) {
     uint32_t o[16];
+    __syncwarp();
     if (any) {
       tmem_ld16_nowait(taddr + col0 + q * 16, o);
       tmem_wait_ld();
