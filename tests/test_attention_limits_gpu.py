@@ -267,3 +267,35 @@ def test_a_failure_is_reported_to_every_thread_once(monkeypatch):
         with pytest.raises(_lib.NativeKernelError):
             pool.submit(other).result()
         assert torch.equal(pool.submit(other).result(), want)
+
+
+@pytest.mark.parametrize("h, hk, n", [(8, 1, 900), (16, 2, 640), (65, 1, 300), (3, 3, 1)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_fp16_small_gradients_of_grouped_heads(h, hk, n, causal):
+    """Query tiles split between blocks, groups that do not divide a tile, and K and V that are views of one
+    projection."""
+    from fast_trimul_b200.functional import packed_attention
+    r, d = gen(12), 64
+    q, kv, g = r(n, h, d).to(HF), r(n, 2, hk, d).to(HF), (1e-3 * r(n, h, d)).to(HF)
+    k, v = kv.unbind(1)
+    got = train(packed_attention, (q, k, v), g, ends([n]), causal=causal)
+    keep = torch.ones(n, n, dtype=torch.bool, device="cuda")
+    x = [t.transpose(0, 1) for t in (q, k, v, g)]
+    x[1], x[2] = (t.repeat_interleave(h // hk, 0) for t in x[1:3])
+    want = list(exact(*x, keep=keep.tril() if causal else keep))
+    want[1:] = [t.unflatten(0, (hk, h // hk)).sum(1) for t in want[1:]]
+    for name, a, b in zip(("dq", "dk", "dv"), got[1:], want):
+        b = b.transpose(0, 1)
+        if n == 1:         # one key, whose weight is 1 whatever q and k: dv is g, and dS what fp32 leaves of 0
+            assert torch.equal(a, g) if name == "dv" else (a.double() - b).abs().max() <= 2 ** -14 * 1e-3 * 64 * 16
+            continue
+        assert roundings(a, b) <= MOST, name
+
+
+def test_fp16_gradients_of_zeros():
+    from fast_trimul_b200.functional import packed_attention
+    q, k, v, g = (gen(13)(70, 2, 32).to(HF) for _ in range(4))
+    cu, zero = ends([40, 30]), torch.zeros_like(q)
+    assert all((t == 0).all() for t in train(packed_attention, (q, k, v), zero, cu)[1:])
+    got = train(packed_attention, (q, k, zero), g, cu)
+    assert (got[1] == 0).all() and (got[2] == 0).all() and not got[3].isnan().any() and (got[3] != 0).any()
