@@ -436,8 +436,8 @@ bool plain(const Tensor& q, const Tensor& k, const Tensor& v, double scale, int6
     return false;
   const int d = q.get_device();
   if (d >= kMaxGpus || !words[d].dev || *words[d].host || !knows_all(d)) return false;
-  return heads % kv_heads == 0 && heads / kv_heads <= 128 && dim % 8 == 0 && dim <= 128 && ready(q) && ready(k) &&
-         ready(v);
+  return heads <= INT_MAX && heads % kv_heads == 0 && heads / kv_heads <= 128 && dim % 8 == 0 && dim <= 128 &&
+         ready(q) && ready(k) && ready(v);
 }
 bool index_ok(const Tensor& t, const Tensor& q) {
   return t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && t.device() == q.device();
@@ -454,7 +454,8 @@ py::object packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   if (q.dim() != 3 || k.dim() != 3 || v.dim() != 3 || q.size(2) != k.size(2)) return py::none();
   const double s = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2)));
   if (k.size(1) < 1 || !plain(q, k, v, s, q.size(1), k.size(1), q.size(2)) || !index_ok(cu_q, q) ||
-      !index_ok(cu_k, q) || cu_q.size(0) != cu_k.size(0) || cu_q.size(0) < 2 || !mask_ok(mask, q, {k.size(0)}))
+      !index_ok(cu_k, q) || cu_q.size(0) != cu_k.size(0) || cu_q.size(0) < 2 || cu_q.size(0) > INT_MAX ||
+      !mask_ok(mask, q, {k.size(0)}))
     return py::none();
   Call c;
   c.seqs = static_cast<int>(cu_q.size(0) - 1);
@@ -474,7 +475,7 @@ py::object cached(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
     return py::none();
   const double s = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2)));
   if (k.size(2) < 1 || !plain(q, k, v, s, q.size(1), k.size(2), q.size(2)) || !index_ok(lengths, q) ||
-      lengths.size(0) != q.size(0))
+      lengths.size(0) != q.size(0) || q.size(0) > INT_MAX)
     return py::none();
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) return py::none();
   Call c;

@@ -299,3 +299,13 @@ def test_fp16_gradients_of_zeros():
     assert all((t == 0).all() for t in train(packed_attention, (q, k, v), zero, cu)[1:])
     got = train(packed_attention, (q, k, zero), g, cu)
     assert (got[1] == 0).all() and (got[2] == 0).all() and not got[3].isnan().any() and (got[3] != 0).any()
+
+
+def test_more_sequences_than_32_bits_count_are_refused():
+    from fast_trimul_b200 import _lib
+    from fast_trimul_b200.functional import packed_attention
+    q = gen(14)(8, 2, 32).to(BF)
+    cu = torch.zeros(2 ** 32 + 3, dtype=torch.int32, device="cuda")      # cut to 32 bits: two sequences
+    cu[-1] = 8
+    with pytest.raises(_lib.NativeDeclined):
+        packed_attention(q, q, q, cu)
