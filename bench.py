@@ -546,7 +546,8 @@ def reference_gpu_subprocess(ns=(64, 128, 256, 2048), timeout_s=300):
 def bench_trunk(args, torch, dev, n=384, blocks=8):
     """The trunk configuration: 8 PairFormer-style blocks, N=384, c_s=384, c_z=128, bf16,
     all-ones masks, random weights; ms per trunk forward with plain-PyTorch TriMul
-    layers vs with FastTriangleMultiplication, everything else identical."""
+    layers vs with FastTriangleMultiplication, everything else identical, and with the
+    library's layer norms and attentions as well (`fused`)."""
     from fast_trimul_b200.pairformer import (PairFormerTrunk, copy_trimul_weights, fast_trimul,
                                              torch_trimul, trunk_flops_trimul)
     torch.manual_seed(0)
@@ -556,6 +557,11 @@ def bench_trunk(args, torch, dev, n=384, blocks=8):
         if hasattr(m, "_impl"):
             m._impl.half()                      # the TriMul weights stay fp16, as in the reference
     copy_trimul_weights(ref, fast)
+    fused = PairFormerTrunk(blocks, 384, C, fast_trimul, fused=True).to(dev).to(torch.bfloat16).eval()
+    for m in fused.modules():
+        if hasattr(m, "_impl"):
+            m._impl.half()
+    fused.load_state_dict(fast.state_dict())
     gen = torch.Generator(device=dev).manual_seed(3)
     s = torch.randn(1, n, 384, device=dev, generator=gen).to(torch.bfloat16)
     z = torch.randn(1, n, n, C, device=dev, generator=gen).to(torch.bfloat16)
@@ -596,17 +602,19 @@ def bench_trunk(args, torch, dev, n=384, blocks=8):
 
     ms_ref, (s_ref, z_ref) = timed(ref)
     ms_fast, (s_fast, z_fast) = timed(fast)
+    ms_fused, (s_fused, z_fused) = timed(fused)
     tri_ref, tri_fast = trimul_layers_ms(ref), trimul_layers_ms(fast)
-    dz = ((z_fast.float() - z_ref.float()).abs().mean() / z_ref.float().abs().mean()).item()
+    rel = lambda z: ((z.float() - z_ref.float()).abs().mean() / z_ref.float().abs().mean()).item()   # noqa: E731
     return {"config": "C4 PairFormer-style trunk, 8 blocks, N=384, c_s=384, c_z=128, bf16",
             "ms_per_fwd_torch_trimul": round(ms_ref, 3), "ms_per_fwd_fast_trimul": round(ms_fast, 3),
+            "ms_per_fwd_fused": round(ms_fused, 3),   # fast TriMul, layer norms and attentions of the library
             "speedup": round(ms_ref / ms_fast, 3),
             "trimul_layers_ms": {"torch": round(tri_ref, 3), "fast": round(tri_fast, 3)},
             "trimul_share_of_trunk": {"torch": round(tri_ref / ms_ref, 3),
                                       "fast": round(tri_fast / ms_fast, 3)},
             "mask_semantics": "both trunks: z * mask before the input LayerNorm, output * mask",
             "trimul_tflop_per_fwd": round(trunk_flops_trimul(n, C, blocks) / 1e12, 4),
-            "z_out_mean_rel_diff": round(dz, 5)}
+            "z_out_mean_rel_diff": round(rel(z_fast), 5), "z_out_mean_rel_diff_fused": round(rel(z_fused), 5)}
 
 
 def bench_e2e(args, torch, layer, dev, n):
