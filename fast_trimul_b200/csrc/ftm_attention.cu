@@ -12,8 +12,10 @@
 // Roles of a block: warps 0-3 softmax and epilogue, warp 4 TMA, warp 5 MMA. Two blocks
 // per SM (256 TMEM columns each: S / P 128, O up to 128), so one block's MMAs run under the
 // other's exponentials. A 128 x 128 tile costs 8 dim clocks of MMA and 1024 clocks of the
-// special function unit, so dim 128 is balanced between the two and smaller heads are
-// bound by the exponentials.
+// special function unit, so dim 128 is balanced between the two, and for smaller heads the
+// exponentials are the floor. Neither bounds the kernel: at N = 384, 4 heads of 32, the counters
+// show 39 % of the exponentials' rate and 14 % of the matrix instructions', and warps that wait
+// for their own last result.
 //
 // Measured, bf16: 2 sequences of 8192 tokens, 16 heads, dim 128, 1000 us (1100 TFLOP/s);
 // one of them, causal, 300 us (917); triangle attention at N = 384, 4 heads of 32, 149 us, the

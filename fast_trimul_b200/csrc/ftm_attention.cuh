@@ -268,11 +268,11 @@ constexpr int kBlk = kTileRows * 128;   // bytes of one 64-element block
 // election among some of them would pick another lane, whose commits do not cover the MMAs of
 // the first one.
 // E: which of the two. The kernels with a bias at DP = 128 keep lane 0: with the election they once
-// ended with an illegal address whose cause is not known. It was none of the addresses: their
-// matrix instructions take the same ones as without a bias at DP = 128, where the elected form
-// runs, and a check of every descriptor and TMEM address found none out of range. Lanes that a
-// branch had parted could then reach TMEM accesses one after the other, which is undefined; that is
-// mended in all kernels. The kernels with a bias stay in the form that was tested.
+// ended with an illegal address whose cause is not known. A check of every descriptor and TMEM
+// address found none out of range, and those of the forward, dq and dkv are the same without a
+// bias, where the elected form runs. Lanes that a branch had parted could then reach TMEM accesses
+// one after the other, which is undefined; that is mended in all kernels. The kernels with a bias
+// stay in the form that was tested.
 template <bool E>
 __device__ __forceinline__ bool issuer(int lane) {
   if (!E) return lane == 0;

@@ -138,7 +138,8 @@ BwdSpace bwd_space(const ftm_attention* p, int want_dbias, int sms) {
   // Few key tiles (one key / value head, a few thousand keys) leave SMs idle: the query tiles of
   // each are split over up to 8 blocks, at least 4 tiles each, and the parts added up. One
   // sequence of 2319 tokens, 8 heads on one, dim 128: the training step 370 us unsplit, 148 us
-  // with the parts and their sums.
+  // with the parts and their sums. (That shape is the rule's only measurement; it goes by the average
+  // length, so that one long sequence among many short ones may stay unsplit.)
   const int64_t tq = kTileRows / (p->heads / p->kv_heads);
   const int64_t k_items = (p->cu_q ? p->kv_rows / kTileRows + p->sequences
                                    : int64_t(p->sequences) * ((p->kv_len + kTileRows - 1) / kTileRows)) * p->kv_heads;

@@ -46,8 +46,11 @@ constexpr int kTmaWarp = 16, kMmaWarp = 17, kElemWarps = 16;
 // out again; it enters exponents and constants that are there anyway. Weights are at most 1 (1.02
 // where a bias puts the scores far from 0): P^T of dkv times 2^14. |dp - d| <= |g| (|v| + |o|), and o
 // is a mean of rows of V: times 2^lift(|g|, largest |v|), |.| the norm of a row, dS stays below
-// 2^15.1. dq takes each row's own |g|; dkv, whose sums run over queries, the largest. 4096 keys, dim
-// 64, gradients of 1e-3: dq was off by 8 times the rounding of the result, now 1.4. bf16 has the
+// 2^15.1. dq takes each row's own |g|; dkv, whose sums run over queries, the largest of the call,
+// which leaves dS of evenly spread weights 13 binades above 2^-14 at 4096 keys: queries whose
+// gradients are more than 2^13 below the largest, or beside one outlier of V, give up bits of dk
+// again. 4096 keys, dim 64: dq was off by 2.8 times the rounding of the result at gradients of 1e-2
+// and by 8 at 1e-3, now by 1.42 and 1.05 (there the result itself is subnormal). bf16 has the
 // exponents of fp32 and needs none of this. It costs fp16 3 to 4 % of a step (ragged batch of 8192
 // rows, 12 heads on 6 of 64: 289 -> 300 us; one sequence of 8192, 16 on 4 of 128: 1550 -> 1586).
 constexpr int kLiftP = 14;
