@@ -29,11 +29,12 @@ int check(const ftm_attention* p) {
   if (p->head_dim < 8 || p->head_dim > 128 || p->head_dim % 8) return FTM_BAD_SHAPE;
   if (p->sequences < 1 || p->q_rows < 1 || p->kv_rows < 1 || p->q_rows > kMaxRows || p->kv_rows > kMaxRows)
     return FTM_BAD_SHAPE;
-  // item numbers are 32-bit too: tiles of either side times heads
+  // item numbers are 32-bit too: tiles of either side times heads (of a cache: of every sequence)
   const int64_t q_tiles = p->q_rows / (kTileRows / (p->heads / p->kv_heads)) + p->sequences;
   const int64_t k_tiles = p->kv_rows / kTileRows + 1;
   if (q_tiles * p->kv_heads > kMaxRows ||
-      (k_tiles + p->sequences) * p->kv_heads * (p->kv_lengths ? p->sequences : 1) > kMaxRows)
+      (p->kv_lengths ? k_tiles * p->kv_heads > kMaxRows / p->sequences
+                     : (k_tiles + p->sequences) * p->kv_heads > kMaxRows))
     return FTM_BAD_SHAPE;
   if (p->kv_lengths) {
     if (p->cu_q || p->cu_k || p->key_mask || p->bias || p->causal || p->stats || p->out_low) return FTM_BAD_ARGUMENT;

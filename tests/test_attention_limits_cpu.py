@@ -148,3 +148,22 @@ def test_the_host_word_is_cleared_last(error_word):
     with pytest.raises(_lib.NativeKernelError):
         w.poll()
     assert done == ["synchronize", "zero", "synchronize", "clear"] and w.word.now == 0
+
+
+def test_large_batches_of_a_cache_are_not_refused():
+    """Items of a cache are its tiles times heads times sequences: sequences were counted twice, and 16 384
+    sequences of 8 heads refused; and a product past 64 bits must not wrap to a small one."""
+    from fast_trimul_b200 import _lib
+    lib, p = _lib.load(), 1 << 20
+
+    def taken(sequences, heads, capacity):
+        a = _lib.Attention(dtype=_lib.BF16, heads=heads, kv_heads=heads, head_dim=64, scale=0.125, sequences=sequences,
+                           q_len=1, q_rows=sequences, kv_rows=capacity, kv_lengths=p, q=p, q_row_stride=64 * heads,
+                           q_head_stride=64, k=p, k_row_stride=64 * heads, k_head_stride=64,
+                           k_batch_stride=64 * heads * capacity, v=p, v_row_stride=64 * heads, v_head_stride=64,
+                           v_batch_stride=64 * heads * capacity, out=p)
+        return lib.ftm_attention_workspace_bytes(a, 0) > 0      # 0: refused
+
+    assert taken(16, 8, 16384) and taken(16384, 8, 4096) and taken(6000, 64, 512)
+    assert not taken(1 << 20, 64, 4096)                         # 2^31 items
+    assert not taken(2 ** 31 - 2048, 1 << 30, 256)

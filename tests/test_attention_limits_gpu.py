@@ -309,3 +309,14 @@ def test_more_sequences_than_32_bits_count_are_refused():
     cu[-1] = 8
     with pytest.raises(_lib.NativeDeclined):
         packed_attention(q, q, q, cu)
+
+
+def test_cached_a_batch_of_many_sequences():
+    """Each (sequence, head) is one tile here, so the same bits as in small batches."""
+    from fast_trimul_b200.functional import cached_attention
+    r, n = gen(15), 16384
+    q, k, v = r(n, 16, 8).to(BF), r(n, 40, 8, 8).to(BF), r(n, 40, 8, 8).to(BF)
+    lens = torch.arange(n, device="cuda", dtype=torch.int32) % 41
+    got = cached_attention(q, k, v, lens)
+    for at in (slice(0, 500), slice(8000, 8300), slice(n - 77, n)):
+        assert torch.equal(got[at], cached_attention(q[at], k[at], v[at], lens[at]))
